@@ -121,7 +121,7 @@ def _prepare_sample(c, gen):
     n, v = c["rows"], c["vocab"]
     logits = torch.randn(n, v, device="cuda", generator=gen) * 2.5
     # a trained model puts most of a row's mass on some tokens
-    top = torch.randint(0, v, (n, 24), device="cuda", generator=gen)
+    top = torch.randint(0, v // 24, (n, 24), device="cuda", generator=gen) + torch.arange(24, device="cuda") * (v // 24)
     logits.scatter_add_(1, top, torch.rand(n, 24, device="cuda", generator=gen) * 10)
     s = {"op": c["op"], "logits": logits.to(DTYPES[c["dtype"]]),
          "u": torch.rand(n, device="cuda", generator=gen)}
@@ -308,7 +308,9 @@ def _append(codes, scales, new, start, counts):
     s5 = scale[..., None, None]
     value = torch.where(is_new, fresh, torch.where(is_old, old_codes.float() * old_scale[..., None, None], 0.0))
     value = (value / s5).clamp(-448, 448).to(codes.dtype).view(torch.uint8)
-    value = torch.where(valid[:, :, None, None, None], value, old_codes.view(torch.uint8))
+    # codes behind the last new token stay as they were
+    touched = valid[:, :, None, None, None] & (is_new | is_old)
+    value = torch.where(touched, value, old_codes.view(torch.uint8))
     scale = torch.where(valid[:, :, None], scale, old_scale)
     # a window that is not valid repeats the first one's outcome
     value = torch.where(valid[:, :, None, None, None], value, value[:, :1])
@@ -445,17 +447,17 @@ def _exact_cache(s):
             end = at + (int(s["counts"][i]) if s["counts"] is not None else n)
             for blk in range(at // BLOCK, -(-min(end, cap) // BLOCK)):
                 lo, hi = blk * BLOCK, min((blk + 1) * BLOCK, end)
-                value = torch.zeros(h, BLOCK, d, dtype=torch.float64, device=codes.device)
+                value = torch.zeros(h, hi - lo, d, dtype=torch.float64, device=codes.device)
                 began, grow = max(at, lo), torch.full((h,), 2.0 ** E_MIN, dtype=torch.float64, device=codes.device)
                 if at > lo:
                     grow = scale[i, :, blk].clone()
                     value[:, :at - lo] = codes[i, :, blk, :at - lo] * grow[:, None, None]
                 fresh = s[name][i, :, began - at:hi - at].double()
-                value[:, began - lo:hi - lo] = fresh
+                value[:, began - lo:] = fresh
                 big = fresh.abs().amax((1, 2))
                 need = torch.exp2(torch.ceil(torch.log2(big / 448)))
                 grow = torch.maximum(grow, torch.where(big > 0, need, 2.0 ** E_MIN))
-                codes[i, :, blk] = _round_e4m3(value / grow[:, None, None])
+                codes[i, :, blk, :hi - lo] = _round_e4m3(value / grow[:, None, None])
                 scale[i, :, blk] = grow
         got[name + "_scale"] = scale
         got[name] = codes.view(b, h, cap, d) if name == "k" else codes.transpose(-1, -2).contiguous()
