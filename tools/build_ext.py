@@ -42,6 +42,11 @@ def build(force: bool = False) -> Path:
         "-D_GLIBCXX_USE_CXX11_ABI=1", "-DHIP_ENABLE_WARP_SYNC_BUILTINS=1",
         f"-I{inc1}", f"-I{inc2}", f"-I{pyinc}", f"-I{CSRC}",
         "-Wno-unused-result", "-Wno-switch-bool",
+        # no packed fp32 arithmetic (v_pk_add/mul/fma_f32): some forms of it
+        # have given wrong results on this hardware without an error, and
+        # -O3 makes them from ordinary float code.  (The host pass warns that
+        # it does not know the feature: harmless.)
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
 
     objs = []
