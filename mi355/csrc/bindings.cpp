@@ -78,6 +78,20 @@ std::vector<torch::Tensor> attn_bwd_v3(torch::Tensor dout, torch::Tensor q, torc
                                        bool causal, bool need_dbias,
                                        double p_drop, c10::optional<torch::Tensor> seed,
                                        c10::optional<torch::Tensor> packed);
+torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps,
+                        torch::Tensor row_exp);
+void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tensor vc,
+                torch::Tensor ks, torch::Tensor vs, c10::optional<torch::Tensor> starts, long start,
+                c10::optional<torch::Tensor> counts);
+torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks,
+                       torch::Tensor vs, c10::optional<torch::Tensor> lengths, long length,
+                       long max_len, c10::optional<torch::Tensor> bias,
+                       c10::optional<torch::Tensor> kpad, double scale);
+torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
+                            c10::optional<torch::Tensor> temperatures, double temperature,
+                            c10::optional<torch::Tensor> top_ks, long top_k,
+                            c10::optional<torch::Tensor> top_ps, double top_p,
+                            c10::optional<torch::Tensor> min_ps, double min_p, long empty_token);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
@@ -121,5 +135,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("v"), py::arg("o"), py::arg("lse"), py::arg("bias"),
         py::arg("kpad"), py::arg("causal"), py::arg("need_dbias"),
         py::arg("p_drop"), py::arg("seed"), py::arg("packed") = c10::nullopt);
+  m.def("w4_linear", &w4_linear);
+  m.def("kv8_append", &kv8_append);
+  m.def("kv8_attn", &kv8_attn);
+  m.def("sample_tokens", &sample_tokens);
   m.attr("__gfx__") = "gfx950";
 }

@@ -238,7 +238,10 @@ class _MfmaLinear(torch.autograd.Function):
 def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """F.linear (no bias) with per-shape dispatch to the hand-written MFMA
     GEMM kernels (see _MfmaLinear). MI355_GEMM_2S=1 opts into the two-stream
-    backward (measured a ~3% LOSS at B=2 — kept for A/B only)."""
+    backward (measured a ~3% LOSS at B=2 — kept for A/B only). A W4Weight
+    goes to linear_w4."""
+    if isinstance(w, W4Weight):
+        return linear_w4(x, w)
     if x.is_cuda and x.dtype in (torch.bfloat16, torch.float16):
         M = x.numel() // x.shape[-1]
         N, K = w.shape
@@ -839,3 +842,10 @@ def seg_postprocess(logits, size):
     if _use_hip(logits):
         return _load_ext().seg_postprocess(logits, int(size[0]), int(size[1]))
     return torch_ref.seg_postprocess(logits, size)
+
+
+# --------------------------------------------------------------------------- #
+# Token step of a served model: 4-bit weights, 8-bit cache, sampling          #
+# --------------------------------------------------------------------------- #
+from .token_step import (KVCache8, W4Weight, decode_attention_kv8,  # noqa: E402,F401
+                         kv8_append, linear_w4, quantize_w4, sample_tokens)

@@ -129,3 +129,159 @@ def seg_postprocess(logits: torch.Tensor, size) -> torch.Tensor:
     up = F.interpolate(logits.float(), size=size, mode="bilinear",
                        align_corners=False)
     return up.argmax(dim=1).to(torch.int32)
+
+
+# --------------------------------------------------------------------------- #
+# 4-bit weights                                                               #
+# --------------------------------------------------------------------------- #
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def w4_dequantize(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    """(N, K/2) codes and (N, K/32) exponents -> fp32 (N, K)."""
+    n, half = codes.shape
+    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
+    nibbles = torch.stack([codes & 15, codes >> 4], -1).view(n, 2 * half)
+    scale = torch.ldexp(torch.ones((), device=codes.device), exps.int() - 127)
+    return (table[nibbles.int()].view(n, -1, 32) * scale[..., None]).view(n, -1)
+
+
+def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    n, k = weight.shape
+    w = weight.float().view(n, -1, 32)
+    amax = w.abs().amax(-1, keepdim=True)
+    # 6 * 2^e >= amax for the upper of the two powers of two
+    _, e = torch.frexp(amax / 6)
+    e = torch.where(amax > 0, e, -126)
+    # halfway values go to the even code, as the format's rounding has it
+    edges = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device=w.device)
+    table = torch.tensor(E2M1, device=w.device)
+    best = None
+    for less in (0, 1):
+        ee = (e - less).clamp(-126, 126)
+        scaled = torch.ldexp(w, -ee)
+        up = torch.bucketize(scaled.abs(), edges, right=True)    # ties up
+        down = torch.bucketize(scaled.abs(), edges)              # ties down
+        code = torch.where(up % 2 == 0, up, down)
+        err = ((table[code] - scaled.abs()) * torch.ldexp(torch.ones_like(amax), ee)).square().sum(-1, keepdim=True)
+        code = code + 8 * (scaled < 0)
+        if best is None:
+            best = (err, code, ee)
+        else:
+            take = err < best[0]
+            best = (None, torch.where(take, code, best[1]), torch.where(take, ee, best[2]))
+    code = best[1].view(n, k).to(torch.uint8)
+    return code[:, 0::2] | code[:, 1::2] << 4, (best[2].view(n, -1) + 127).to(torch.uint8)
+
+
+def linear_w4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    acc = x.dtype if x.dtype == torch.float64 else torch.float32
+    return torch.matmul(x.to(acc), w4_dequantize(codes, exps).to(acc).t()).to(x.dtype)
+
+
+# --------------------------------------------------------------------------- #
+# key/value cache in 8 bits                                                   #
+# --------------------------------------------------------------------------- #
+KV8_BLOCK, KV8_E_MIN, KV8_E_MAX = 64, -120, 120
+
+
+def kv8_scale(amax: torch.Tensor) -> torch.Tensor:
+    """2^ceil(log2(amax / 448)), within the exponents a scale may have."""
+    f, e = torch.frexp(amax)                       # amax = f 2^e, f in [0.5, 1)
+    e = e - 9 + (f > 0.875).to(e.dtype)            # 448 = 0.875 * 2^9
+    e = torch.where(amax > 0, e.clamp(KV8_E_MIN, KV8_E_MAX), KV8_E_MIN)
+    return torch.ldexp(torch.ones_like(amax), e)
+
+
+def kv8_values(k, v, k_scale, v_scale) -> tuple[torch.Tensor, torch.Tensor]:
+    b, h, cap, d = k.shape
+    kf = (k.float().view(b, h, -1, KV8_BLOCK, d) * k_scale[..., None, None]).view(b, h, cap, d)
+    vf = (v.float() * v_scale[..., None, None]).transpose(-1, -2).reshape(b, h, cap, d)
+    return kf, vf
+
+
+def kv8_append(kc, vc, k_scale, v_scale, k, v, start, counts=None) -> None:
+    b, h, cap, d = kc.shape
+    for codes, scales, new in ((kc.view(b, h, -1, KV8_BLOCK, d), k_scale, k),
+                               (vc.transpose(-1, -2), v_scale, v)):
+        for i in range(b):
+            at = int(start[i]) if torch.is_tensor(start) else start
+            n = min(int(counts[i]), new.shape[2]) if counts is not None else new.shape[2]
+            if at < 0 or n <= 0:
+                continue
+            end = min(at + n, cap)
+            for blk in range(at // KV8_BLOCK, -(-end // KV8_BLOCK)):
+                base = blk * KV8_BLOCK
+                lo, hi = max(at - base, 0), min(end - base, KV8_BLOCK)
+                fresh = new[i, :, base + lo - at:base + hi - at].float()      # (H, n, D)
+                size = torch.where(fresh.abs() < math.inf, fresh.abs(), 0.0)
+                scale = kv8_scale(size.amax((1, 2)))
+                if lo > 0:
+                    old = scales[i, :, blk]
+                    scale = torch.maximum(scale, old)
+                    ratio = (old / scale)[:, None, None]
+                    kept = codes[i, :, blk, :lo].float() * ratio
+                    codes[i, :, blk, :lo] = kept.to(codes.dtype)
+                codes[i, :, blk, lo:hi] = (fresh / scale[:, None, None]).clamp(-448, 448).to(codes.dtype)
+                scales[i, :, blk] = scale
+
+
+def decode_attention_kv8(q, k, v, k_scale, v_scale, lengths, bias, kpad, scale, max_len):
+    b, h, cap, d = k.shape
+    kf, vf = kv8_values(k, v, k_scale, v_scale)
+    kf, vf = kf[:, :, :max_len], vf[:, :, :max_len]
+    there = torch.arange(max_len, device=q.device) < (
+        lengths[:, None] if torch.is_tensor(lengths) else torch.full((b, 1), lengths, device=q.device))
+    if kpad is not None:
+        there = there & (kpad[:, :max_len] != -math.inf)
+    # what is not there counts for nothing, whatever it holds
+    kf = torch.where(there[:, None, :, None], kf, 0.0)
+    vf = torch.where(there[:, None, :, None], vf, 0.0)
+    s = torch.matmul(q.float().reshape(b, h, -1, d), kf.transpose(-1, -2).contiguous()) * scale
+    if bias is not None:
+        s = s + bias[..., :max_len].float().reshape(bias.shape[0], h, -1, max_len)
+    if kpad is not None:
+        s = s + kpad[:, None, None, :max_len].float()
+    s = torch.where(there[:, None, None], s, -math.inf)
+    if max_len == 0:
+        return torch.zeros_like(q)
+    m = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
+    l = p.sum(-1, keepdim=True)
+    o = torch.where(l == 0, 0.0, torch.matmul(p, vf) / l)
+    return o.reshape(b, -1, 1, d).to(q.dtype)
+
+
+# --------------------------------------------------------------------------- #
+# choosing a token                                                            #
+# --------------------------------------------------------------------------- #
+def sample_tokens(logits, u, temperature, top_k, top_p, min_p, empty_token: int = -1):
+    x = logits.double()
+    x = torch.where(torch.isnan(x), -math.inf, x)
+
+    def column(v, dtype):
+        return v.to(dtype)[:, None] if torch.is_tensor(v) else \
+            torch.full((len(x), 1), v, device=x.device, dtype=dtype)
+
+    t, k = column(temperature, torch.float64), column(top_k, torch.int64)
+    p, floor = column(top_p, torch.float64), column(min_p, torch.float64).clamp(max=1.0)
+    greedy = ~(t > 0)
+    k = torch.where(greedy, 1, torch.where(k <= 0, x.shape[1], k))
+    t = torch.where(greedy, 1.0, t)
+    m = x.amax(1, keepdim=True)
+    w = torch.where(x == m, 1.0, torch.exp((x - m) / t))
+    w = torch.where((m == -math.inf) | (w < 2.0 ** -45), 0.0, w)
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices
+    rank = torch.arange(x.shape[1], device=x.device)[None]
+    ws = torch.where(rank < k, w.gather(1, order), 0.0)
+    cum = ws.cumsum(1)
+    before = torch.nn.functional.pad(cum[:, :-1], (1, 0))
+    keep = (rank < k) & ((rank == 0) | ~(p < 1) | (before < p * cum[:, -1:])) & ~(ws < floor)
+    kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, ws, 0.0))
+    cum = kept.cumsum(1)
+    r = u.double().clamp(min=0.0)[:, None] * cum[:, -1:]
+    over = (cum > r) & (kept > 0)
+    # u = 1 (or a rounding of u times the sum): the last one kept
+    ids = torch.where(over.any(1), over.to(torch.int8).argmax(1),
+                      x.shape[1] - 1 - (kept > 0).to(torch.int8).flip(1).argmax(1))
+    return torch.where(cum[:, -1] > 0, ids, empty_token)
