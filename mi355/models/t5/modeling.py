@@ -57,6 +57,13 @@ def relative_position_bucket(rel_pos: torch.Tensor, bidirectional: bool,
     return ret + torch.where(is_small, n, val_large)
 
 
+def _linear(x, weight):
+    """F.linear (no bias), or the 4-bit product where the weight was quantized."""
+    if isinstance(weight, ops.W4Weight):
+        return ops.linear_w4(x, weight)
+    return F.linear(x, weight)
+
+
 class _FusedLinears(nn.Module):
     """N same-shaped bias-free projections stored as ONE fused weight so the
     forward is a single hipBLASLt GEMM (q/k/v -> 1 GEMM, wi_0/wi_1 -> 1 GEMM:
@@ -71,10 +78,13 @@ class _FusedLinears(nn.Module):
         self.weight = nn.Parameter(torch.empty(len(self.names) * d_out, d_in))
 
     def forward(self, x):
-        y = F.linear(x, self.weight)
+        y = _linear(x, self.weight)
         return y.split(self.d_out, dim=-1)
 
     def part(self, i):
+        if isinstance(self.weight, ops.W4Weight):
+            return self.weight if len(self.names) == 1 else \
+                self.weight.rows(i * self.d_out, (i + 1) * self.d_out)
         return self.weight[i * self.d_out:(i + 1) * self.d_out]
 
 
@@ -166,13 +176,13 @@ class T5Attention(nn.Module):
 
     # q/k/v as single projections (cross-attention + generate cache paths)
     def q(self, x):
-        return F.linear(x, self.qkv.part(0))
+        return _linear(x, self.qkv.part(0))
 
     def k(self, x):
-        return F.linear(x, self.qkv.part(1))
+        return _linear(x, self.qkv.part(1))
 
     def v(self, x):
-        return F.linear(x, self.qkv.part(2))
+        return _linear(x, self.qkv.part(2))
 
     def compute_bias(self, sq: int, sk: int, device) -> torch.Tensor:
         """(1, H, sq, sk) additive relative-position bias."""
@@ -201,10 +211,13 @@ class T5Attention(nn.Module):
                 causal=False, kv_cache=None, kv5=None):
         """kv_cache: optional dict used by generate() —
         {"k","v": (B,H,Tmax,D) preallocated, "len": int} for self-attn append,
-        or {"k","v" precomputed static} for cross-attn.
+        or {"k","v" precomputed static} for cross-attn; with "kv8" (a
+        KVCache8) in place of "k","v" the cache is held in 8 bits.
         kv5: (B, Sk, 2, H, D) precomputed packed kv (decoder cross-attention
         with kv_external: one stack-level GEMM feeds every layer)."""
         b, sq, _ = hidden.shape
+        if kv_cache is not None and "kv8" in kv_cache:
+            return self._decode_kv8(hidden, position_bias, kpad, kv_cache)
         static = kv_cache is not None and kv_cache.get("static", False)
         if kv_hidden is None and kv_cache is None:
             # self-attention without a cache (training / encoder): ONE fused
@@ -264,6 +277,23 @@ class T5Attention(nn.Module):
         return ops.linear(out, self.o.weight)
 
 
+    def _decode_kv8(self, hidden, position_bias, kpad, kv_cache):
+        """One token over an 8-bit cache: {"kv8", "len"}, "static" for the
+        encoder's keys and values, which are not appended to."""
+        b, sq, _ = hidden.shape
+        if sq != 1:
+            raise ValueError(f"an 8-bit cache takes one token at a time, got {sq}")
+        if kv_cache.get("static", False):
+            q = self._shape(self.q(hidden), b)
+        else:
+            q, k, v = (self._shape(t, b) for t in self.qkv(hidden))
+            ops.kv8_append(kv_cache["kv8"], k, v, kv_cache["len"])
+            kv_cache["len"] += 1
+        out = ops.decode_attention_kv8(q, kv_cache["kv8"], kv_cache["len"],
+                                       bias=position_bias, kpad=kpad)
+        return ops.linear(out.transpose(1, 2).reshape(b, sq, self.inner_dim), self.o.weight)
+
+
 class T5LayerSelfAttention(nn.Module):
     def __init__(self, config, has_relative_attention_bias, is_decoder):
         super().__init__()
@@ -306,7 +336,7 @@ class T5DenseGatedActDense(nn.Module):
         # fused on its output (no gate/up split views, no grad cat)
         p = self.dropout.p if self.training else 0.0
         h = ops.geglu_packed(ops.linear(x, self.wi.weight), p_drop=p,
-                             salt=self.wi.weight.data_ptr())
+                             salt=self.wi.weight.data_ptr() if p > 0 else 0)
         return ops.linear(h, self.wo.weight)
 
 
@@ -513,46 +543,119 @@ class T5ForConditionalGeneration(nn.Module):
             loss = ops.cross_entropy(logits, labels, ignore_index=-100)
         return Seq2SeqOutput(loss=loss, logits=logits, encoder_last_hidden_state=encoder_outputs)
 
-    # -- greedy generate with preallocated KV cache -------- #
+    # -- inference in fewer bits -------------------------------------------- #
+    @torch.no_grad()
+    def quantize_decoder_w4(self) -> "T5ForConditionalGeneration":
+        """Replace the weights that every decoded token reads - the decoder's
+        projections and feed-forwards, and an untied lm head - by 4-bit codes
+        (ops.W4Weight, 4.25 bits a weight).  The encoder, the fused cross-
+        attention k/v projection and the embeddings, read once a sequence, keep
+        their type.  In place, and for inference: the decoder cannot be trained
+        or saved afterwards."""
+        linears = [] if self.config.tie_word_embeddings else [self.lm_head]
+        for blk in self.decoder.block:
+            sa, ca, ff = blk.layer[0].SelfAttention, blk.layer[1].EncDecAttention, blk.layer[2].DenseReluDense
+            linears += [sa.qkv, sa.o, ca.qkv, ca.o, ff.wi, ff.wo]
+        for lin in linears:
+            if not isinstance(lin.weight, ops.W4Weight):
+                w4 = ops.quantize_w4(lin.weight)
+                del lin.weight
+                lin.weight = w4
+        self._gen_graph = None   # it holds the old weights
+        return self
+
+    # -- generate with preallocated KV cache (SURVEY.md §3.3) --------------- #
     @torch.no_grad()
     def generate(self, input_ids=None, attention_mask=None, max_new_tokens: int = 128,
                  min_new_tokens: int = 0, eos_token_id=None, use_graph: bool | None = None,
-                 **_ignored):
-        """Greedy decode. On GPU with a fixed token budget
+                 do_sample: bool = False, temperature: float = 1.0, top_k: int = 50,
+                 top_p: float = 1.0, min_p: float = 0.0,
+                 generator: torch.Generator | None = None,
+                 kv_cache_dtype: str | None = None, **_ignored):
+        """Greedy decode, or with ``do_sample`` a token drawn at every step
+        after temperature, top-k, top-p and min-p (ops.sample_tokens; the
+        numbers come from ``generator``, or the device's default one).
+        ``kv_cache_dtype="fp8"`` holds the decoder's caches in 8 bits
+        (ops.KVCache8).  On GPU with a fixed token budget
         (min_new_tokens == max_new_tokens) the whole decode loop is captured
         ONCE as a hipGraph and replayed per call — the loop is launch-bound
         (~90 small kernels per token step) and the replay removes the
         CPU-side gap. Disable with use_graph=False / MI355_GEN_GRAPH=0."""
+        if kv_cache_dtype not in (None, "fp8"):
+            raise ValueError(f"kv_cache_dtype is None or 'fp8', got {kv_cache_dtype!r}")
+        kv8 = kv_cache_dtype == "fp8"
+        dt = self.shared.weight.dtype
+        if input_ids.is_cuda and dt not in (torch.bfloat16, torch.float16) and \
+                (kv8 or isinstance(self.decoder.block[0].layer[2].DenseReluDense.wo.weight, ops.W4Weight)):
+            raise ValueError(f"8-bit caches and 4-bit weights take a bf16 or fp16 model on a GPU, got {dt}")
+        sampling = None
+        if do_sample:
+            sampling = {"temperature": float(temperature), "top_k": int(top_k),
+                        "top_p": float(top_p), "min_p": float(min_p)}
+            ops.check_sampling(**sampling)
         if use_graph is None:
             use_graph = os.environ.get("MI355_GEN_GRAPH", "1") != "0"
         if (use_graph and input_ids.is_cuda and min_new_tokens == max_new_tokens
                 and not self.training):
+            # drawn before the attempt, so that the eager fallback has them too
+            u = self._uniforms(sampling, max_new_tokens, input_ids, generator)
             try:
                 return self._generate_graphed(input_ids, attention_mask, max_new_tokens,
-                                              eos_token_id)
+                                              eos_token_id, sampling, u, kv8)
             except Exception as e:
                 if not getattr(self, "_gen_graph_warned", False):
                     self._gen_graph_warned = True
                     print(f"# decode-graph capture failed, eager fallback: {e!r}")
+        else:
+            u = self._uniforms(sampling, max_new_tokens, input_ids, generator)
         return self._generate_eager(input_ids, attention_mask, max_new_tokens,
-                                    min_new_tokens, eos_token_id)
+                                    min_new_tokens, eos_token_id, sampling, u, kv8)
 
-    def _cross_kv_all(self, enc, b):
+    @staticmethod
+    def _uniforms(sampling, steps, input_ids, generator):
+        """(steps, B) uniform numbers for a call that samples."""
+        if sampling is None:
+            return None
+        return torch.rand(steps, input_ids.shape[0], device=input_ids.device, generator=generator)
+
+    def _pick(self, logits, sampling, u_t):
+        if sampling is None:
+            return logits.argmax(dim=-1)
+        return ops.sample_tokens(logits, u_t, empty_token=self.config.pad_token_id, **sampling)
+
+    def _lm_logits(self, x):
+        if isinstance(self.lm_head.weight, ops.W4Weight):
+            return ops.linear_w4(x, self.lm_head.weight)
+        return self.lm_head(x)
+
+    def _cross_kv_views(self, enc, b):
         """One fused (B*S, n*2*inner) GEMM for every decoder layer's static
-        cross-attention kv; returns (n, 2) nested views shaped (B,H,S,D)."""
+        cross-attention kv; (n, 2) nested views shaped (B,H,S,D)."""
         cfg = self.config
         h, dkv = cfg.num_heads, cfg.d_kv
         n = len(self.decoder.block)
         kv_all = ops.linear(enc, self.decoder.cross_kv).view(
             b, enc.shape[1], n, 2, h, dkv)
-        return [(kv_all[:, :, i, 0].permute(0, 2, 1, 3).contiguous(),
-                 kv_all[:, :, i, 1].permute(0, 2, 1, 3).contiguous())
+        return [(kv_all[:, :, i, 0].permute(0, 2, 1, 3),
+                 kv_all[:, :, i, 1].permute(0, 2, 1, 3))
                 for i in range(n)]
 
-    def _decode_caches(self, enc, b, max_new_tokens, dev, dt):
+    def _cross_kv_all(self, enc, b):
+        return [(k.contiguous(), v.contiguous()) for k, v in self._cross_kv_views(enc, b)]
+
+    def _decode_caches(self, enc, b, max_new_tokens, dev, dt, kv8=False):
         cfg = self.config
         h, dkv = cfg.num_heads, cfg.d_kv
         caches = []
+        if kv8:
+            for _ in self.decoder.block:
+                caches.append({
+                    "self": {"kv8": ops.KVCache8(b, h, max_new_tokens, dkv, device=dev), "len": 0},
+                    "cross": {"kv8": ops.KVCache8(b, h, enc.shape[1], dkv, device=dev),
+                              "len": enc.shape[1], "static": True},
+                })
+            self._fill_cross_kv8(caches, enc, b)
+            return caches
         kv_pairs = self._cross_kv_all(enc, b)
         for i, blk in enumerate(self.decoder.block):
             ck, cv = kv_pairs[i]
@@ -564,9 +667,13 @@ class T5ForConditionalGeneration(nn.Module):
             })
         return caches
 
+    def _fill_cross_kv8(self, caches, enc, b):
+        for cache, (k, v) in zip(caches, self._cross_kv_views(enc, b)):
+            ops.kv8_append(cache["cross"]["kv8"], k, v, 0)
+
     @torch.no_grad()
     def _generate_graphed(self, input_ids, attention_mask, max_new_tokens,
-                          eos_token_id=None):
+                          eos_token_id=None, sampling=None, u=None, kv8=False):
         cfg = self.config
         b = input_ids.shape[0]
         dev = input_ids.device
@@ -577,19 +684,23 @@ class T5ForConditionalGeneration(nn.Module):
         # generations could emit EOS mid-sequence followed by garbage that
         # survives skip_special_tokens decoding.
         eos = cfg.eos_token_id if eos_token_id is None else eos_token_id
-        key = (b, input_ids.shape[1], max_new_tokens, str(dev), eos)
+        key = (b, input_ids.shape[1], max_new_tokens, str(dev), eos, kv8,
+               tuple(sampling.values()) if sampling is not None else None)
         state = getattr(self, "_gen_graph", None)
         kpad = _kpad_from_mask(attention_mask)
         enc = self.encoder(input_ids=input_ids, kpad=kpad)
         if state is None or state["key"] != key or (kpad is None) != (state["kpad"] is None):
             # build static buffers and capture the 128-step decode loop
-            caches = self._decode_caches(enc, b, max_new_tokens, dev, dt)
+            caches = self._decode_caches(enc, b, max_new_tokens, dev, dt, kv8)
+            u_static = u.clone() if u is not None else None
             enc_static = enc.clone()
             kpad_static = kpad.clone() if kpad is not None else None
             out_tokens = torch.zeros(b, max_new_tokens, device=dev, dtype=torch.long)
             attn0 = self.decoder.block[0].layer[0].SelfAttention
             full_bias = attn0.compute_bias(max_new_tokens, max_new_tokens, dev).float()
-            bias_steps = [full_bias[:, :, t:t + 1, :t + 1].contiguous()
+            # the 8-bit path reads the fp32 row in place, behind the length too
+            bias_steps = [full_bias[:, :, t:t + 1] if kv8 else
+                          full_bias[:, :, t:t + 1, :t + 1].contiguous()
                           for t in range(max_new_tokens)]
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
@@ -600,33 +711,40 @@ class T5ForConditionalGeneration(nn.Module):
                     caches[i]["self"]["len"] = 0
                 for t in range(max_new_tokens):
                     dec = self._decode_step(tok, enc_static, kpad_static, caches,
-                                            t, bias_steps[t].to(dt))
+                                            t, bias_steps[t] if kv8 else bias_steps[t].to(dt))
                     if cfg.tie_word_embeddings:
                         dec = dec * (self.model_dim**-0.5)
-                    logits = self.lm_head(dec[:, -1])
+                    logits = self._lm_logits(dec[:, -1])
                     if eos is not None:
                         logits[:, eos] = float("-inf")
-                    nxt = logits.argmax(dim=-1)
+                    nxt = self._pick(logits, sampling, u_static[t] if u is not None else None)
                     out_tokens[:, t] = nxt
                     tok = nxt.unsqueeze(1)
             state = {"key": key, "graph": g, "enc": enc_static, "kpad": kpad_static,
-                     "caches": caches, "out": out_tokens}
+                     "caches": caches, "out": out_tokens, "u": u_static,
+                     "bias": bias_steps}
             self._gen_graph = state
         # refresh the static inputs, reset self-cache lengths, replay
         state["enc"].copy_(enc)
         if kpad is not None:
             state["kpad"].copy_(kpad)
-        kv_pairs = self._cross_kv_all(enc, input_ids.shape[0])
-        for i, blk in enumerate(self.decoder.block):
-            state["caches"][i]["cross"]["k"].copy_(kv_pairs[i][0])
-            state["caches"][i]["cross"]["v"].copy_(kv_pairs[i][1])
-            state["caches"][i]["self"]["len"] = 0
+        if u is not None:
+            state["u"].copy_(u)
+        if kv8:
+            self._fill_cross_kv8(state["caches"], enc, b)
+        else:
+            kv_pairs = self._cross_kv_all(enc, input_ids.shape[0])
+            for i, blk in enumerate(self.decoder.block):
+                state["caches"][i]["cross"]["k"].copy_(kv_pairs[i][0])
+                state["caches"][i]["cross"]["v"].copy_(kv_pairs[i][1])
+                state["caches"][i]["self"]["len"] = 0
         state["graph"].replay()
         return state["out"].clone()
 
     @torch.no_grad()
     def _generate_eager(self, input_ids=None, attention_mask=None, max_new_tokens: int = 128,
-                        min_new_tokens: int = 0, eos_token_id=None, **_ignored):
+                        min_new_tokens: int = 0, eos_token_id=None, sampling=None,
+                        u=None, kv8=False):
         cfg = self.config
         eos = cfg.eos_token_id if eos_token_id is None else eos_token_id
         b = input_ids.shape[0]
@@ -634,7 +752,7 @@ class T5ForConditionalGeneration(nn.Module):
         dt = self.shared.weight.dtype
         kpad = _kpad_from_mask(attention_mask)
         enc = self.encoder(input_ids=input_ids, kpad=kpad)
-        caches = self._decode_caches(enc, b, max_new_tokens, dev, dt)
+        caches = self._decode_caches(enc, b, max_new_tokens, dev, dt, kv8)
         tokens = torch.full((b, 1), cfg.decoder_start_token_id, device=dev, dtype=torch.long)
         out_tokens = []
         finished = torch.zeros(b, dtype=torch.bool, device=dev)
@@ -644,13 +762,14 @@ class T5ForConditionalGeneration(nn.Module):
             # one fp32-contiguous slice per step, shared by all layers (the
             # decode kernel wants f32 bias; avoids 12 per-layer re-copies)
             bias_t = full_bias[:, :, t : t + 1, : t + 1].float().contiguous()
+            u_t = u[t] if u is not None else None
             dec = self._decode_step(tokens, enc, kpad, caches, t, bias_t)
             if cfg.tie_word_embeddings:
                 dec = dec * (self.model_dim**-0.5)
-            logits = self.lm_head(dec[:, -1])
+            logits = self._lm_logits(dec[:, -1])
             if t < min_new_tokens:
                 logits[:, eos] = float("-inf")
-            nxt = logits.argmax(dim=-1)
+            nxt = self._pick(logits, sampling, u_t)
             nxt = torch.where(finished, torch.full_like(nxt, cfg.pad_token_id), nxt)
             out_tokens.append(nxt)
             finished |= nxt == eos
@@ -685,6 +804,9 @@ class T5ForConditionalGeneration(nn.Module):
 
     # -- HF-layout checkpoint I/O --------------------------- #
     def save_pretrained(self, save_dir: str, safe_serialization: bool = True):
+        if any(isinstance(m, ops.W4Weight) for m in self.modules()):
+            raise RuntimeError("a model with 4-bit weights is for inference: save it before "
+                               "quantize_decoder_w4()")
         os.makedirs(save_dir, exist_ok=True)
         self.config.save_pretrained(save_dir)
         state = {k: v for k, v in self.state_dict().items()}

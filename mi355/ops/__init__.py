@@ -847,5 +847,6 @@ def seg_postprocess(logits, size):
 # --------------------------------------------------------------------------- #
 # Token step of a served model: 4-bit weights, 8-bit cache, sampling          #
 # --------------------------------------------------------------------------- #
-from .token_step import (KVCache8, W4Weight, decode_attention_kv8,  # noqa: E402,F401
-                         kv8_append, linear_w4, quantize_w4, sample_tokens)
+from .token_step import (KVCache8, W4Weight, check_sampling,  # noqa: E402,F401
+                         decode_attention_kv8, kv8_append, linear_w4,
+                         quantize_w4, sample_tokens)

@@ -244,6 +244,13 @@ def decode_attention_kv8(q: torch.Tensor, cache: KVCache8, lengths, bias=None, k
 # --------------------------------------------------------------------------- #
 # choosing the token                                                          #
 # --------------------------------------------------------------------------- #
+def check_sampling(temperature, top_k, top_p, min_p) -> None:
+    """Refuse sampling options that are out of range."""
+    if not 0 <= temperature < math.inf or not 0 <= top_p <= 1 or not 0 <= min_p <= 1 or top_k < 0:
+        raise ValueError("sampling: temperature and top_k are at least 0, top_p and min_p from 0 to 1; "
+                         f"got {temperature}, {top_k}, {top_p}, {min_p}")
+
+
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                   min_p=0.0, empty_token: int = -1) -> torch.Tensor:
     """One token a row of logits (B, V) from given uniform numbers u (B,).
@@ -271,9 +278,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     ks, top_k = _per_row(top_k, "top_k", rows, dev, torch.int32)
     ps, top_p = _per_row(top_p, "top_p", rows, dev, torch.float32)
     mins, min_p = _per_row(min_p, "min_p", rows, dev, torch.float32)
-    if not 0 <= temperature < math.inf or not 0 <= top_p <= 1 or not 0 <= min_p <= 1 or top_k < 0:
-        raise ValueError("sample_tokens: temperature and top_k are at least 0, top_p and min_p from 0 to 1; "
-                         f"got {temperature}, {top_k}, {top_p}, {min_p}")
+    check_sampling(temperature, top_k, top_p, min_p)
     top_k = min(top_k, logits.shape[1])
     if not logits.is_cuda or not _use_hip(logits):
         pick = lambda each, one: one if each is None else each  # noqa: E731
