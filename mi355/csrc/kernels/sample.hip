@@ -9,17 +9,23 @@
 // Every cut is a prefix of ONE order, so the kept set is "everything up to a
 // border element (value, index)" and nothing is sorted: a histogram over the
 // distance from the maximum gives the border's bin, the bin's few elements are
-// ranked against each other, and a last pass in index order finds the token.
+// ranked against each other, and the kept ones - usually some hundred - go to a
+// list in LDS that the later steps work on.  If they do not fit, the later
+// steps run over the row again with the border as a filter.
 //
 // A token is a comparison of a sum with as many borders as there are logits:
 // an error e in the cumulative share moves a row's token with a probability of
 // about 2 V e, one row in 150 in fp32 at V = 32128.  So weights are computed in
-// fp64 (table of 2^(j/64) and a polynomial of degree 5, relative error under
-// 1e-14) and summed as integers w * 2^44: exact, in any order, hence atomics
+// fp64 (a table of 2^(j/32) and a polynomial of degree 5; relative error under
+// 1e-14 and that of (x - max)/T) and summed as integers w * 2^44: exact, in any order, hence atomics
 // whose order does not matter.  A weight under 2^-45 counts as none.
 //
-// One workgroup a row; the row is read a few times, from memory once and from
-// the L2 after that.
+// One workgroup a row; the row is read from memory once, and a few times from
+// the L2 after that.  What bounds it is one CU's instruction rate (an
+// instruction for every logit of a 32128 row is 0.2 us; a weight is about 20 of
+// them) and, in code that runs once, instruction fetch: passes over the row are
+// short loops, and what happens to few elements is left to a compact inner loop
+// over a bit mask.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -29,13 +35,19 @@
 namespace {
 
 typedef unsigned long long u64;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = 2 * THREADS;
-constexpr int CAP = THREADS;             // elements of a border bin ranked at once
-constexpr int MAX_V = 1 << 19;           // sums stay under 2^63
-constexpr int SEGS = MAX_V / 512 + 16;   // a wave's 512 logits
-constexpr u64 NO_BORDER = 0;             // below every element
+constexpr int CAP = THREADS;             // elements ranked against each other at once
+constexpr int LIST = 4 * THREADS;        // kept elements that the list holds
+constexpr int SHORT = 192;               // lists up to this are summed pair by pair
+constexpr int FEW = 512;                 // a top-k up to this is found without a histogram of the row
+constexpr int MAX_V = 1 << 19;           // sums of w * 2^44 stay under 2^63
+constexpr int SEG = 512;                 // logits of a segment: a wave's 64 slots of 8
+constexpr int SEGS = MAX_V / SEG;
+constexpr double ONE = 17592186044416.0; // 2^44
+constexpr int TABLE = 32;              // 8 bytes each: one for every pair of LDS banks
 
 struct Opt {                             // a number for all rows, or one each
   const void* each;
@@ -44,368 +56,683 @@ struct Opt {                             // a number for all rows, or one each
   DEVINL int i(int row) const { return each ? ((const int*)each)[row] : (int)all; }
 };
 
-// 2^(j/64), correctly rounded
-__constant__ const double EXP2_64[64] = {
-    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
-    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
-    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
-    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
-    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
-    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
-    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
-    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
-    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
-    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
-    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
-    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
-    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
-    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
-    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
-    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951,
+// The bits of 2^44 * 2^(j/32), correctly rounded, less j << 47: with n << 47
+// added for n = 32 i + j, what stays of it is i in the exponent field.
+__constant__ const u64 EXP2_TABLE[TABLE] = {
+    0x42b0000000000000ull, 0x42afd9b0d3158574ull, 0x42afb5586cf9890full, 0x42af9301d0125b51ull,
+    0x42af72b83c7d517bull, 0x42af54873168b9aaull, 0x42af387a6e756238ull, 0x42af1e9df51fdee1ull,
+    0x42af06fe0a31b715ull, 0x42aef1a7373aa9cbull, 0x42aedea64c123422ull, 0x42aece086061892dull,
+    0x42aebfdad5362a27ull, 0x42aeb42b569d4f82ull, 0x42aeab07dd485429ull, 0x42aea47eb03a5585ull,
+    0x42aea09e667f3bcdull, 0x42ae9f75e8ec5f74ull, 0x42aea11473eb0187ull, 0x42aea589994cce13ull,
+    0x42aeace5422aa0dbull, 0x42aeb737b0cdc5e5ull, 0x42aec49182a3f090ull, 0x42aed503b23e255dull,
+    0x42aee89f995ad3adull, 0x42aeff76f2fb5e47ull, 0x42af199bdd85529cull, 0x42af3720dcef9069ull,
+    0x42af5818dcfba487ull, 0x42af7c97337b9b5full, 0x42afa4afa2a490daull, 0x42afd0765b6e4540ull,
 };
 
-// e^a for a <= 0, zero under -40:  a = n ln2/64 + r,  |r| <= ln2/128
-DEVINL double exp_neg(double a, const double* table) {
-  if (!(a > -40.0)) return 0.0;
-  const double n = __builtin_rint(a * 92.33248261689366);        // 64/ln2
-  double r = __builtin_fma(n, -0.010830424696249145, a);          // ln2/64
-  r = __builtin_fma(n, -3.623510646634843e-19, r);                  // and its rest
-  double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
-  p = __builtin_fma(p, r, 1.0 / 6);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  const int k = (int)n;
-  return __builtin_ldexp(p * table[k & 63], k >> 6);
-}
-
-// a larger float has a larger key; -inf is the lowest of what occurs
-DEVINL unsigned key_of(float x) {
+// A larger float has a larger key; with the index: one order over all elements
+// of a row, larger first, then the lower index.
+DEVINL u64 rank_key(float x, int idx) {
   const unsigned u = __builtin_bit_cast(unsigned, x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (u64)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (unsigned)~idx;
 }
-// one order over all elements of a row: value, then the lower index first
-DEVINL u64 rank_key(float x, int idx) { return (u64)key_of(x) << 32 | (unsigned)~idx; }
+DEVINL float value_of(u64 key) {
+  const unsigned u = (unsigned)(key >> 32);
+  return __builtin_bit_cast(float, u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+DEVINL int index_of(u64 key) { return (int)~(unsigned)key; }
 
+// exp((x - max)/T) * 2^44 as an integer.  y = (x - max) * 32/(T ln2) = n + f,
+// 2^(y/32) = 2^(n/32) * e^(f ln2/32) with |f| <= 1/2.
+struct Weights {
+  double max, slope;
+  float least;         // whose weight is under 2^-46: taken for what is less, and for NaN
+  const u64* table;
+  // the integer in the low 52 bits, under the exponent field of 2^52
+  DEVINL u64 raw(float x) const {
+    const double y = ((double)fmaxf(x, least) - max) * slope;
+    // added to 1.5 * 2^52, y is rounded to the integer in the low bits
+    const double magic = 6755399441055744.0;
+    const double rounded = y + magic;
+    const int n = (int)__builtin_bit_cast(u64, rounded);
+    const double f = y - (rounded - magic);
+    double p = __builtin_fma(f, 3.973709984549416e-11, 9.172562701824643e-09);
+    p = __builtin_fma(p, f, 1.693850972437182e-06);
+    p = __builtin_fma(p, f, 0.0002345961982022468);
+    p = __builtin_fma(p, f, 0.02166084939249829);
+    p = __builtin_fma(p, f, 1.0);
+    const u64 base = table[n & (TABLE - 1)] + ((u64)(unsigned)n << 47);
+    // added to 2^52, the weight is rounded to the integer in the low bits
+    return __builtin_bit_cast(u64, __builtin_fma(p, __builtin_bit_cast(double, base), 4503599627370496.0));
+  }
+  DEVINL u64 of(float x) const { return raw(x) & 0xfffffffffffffull; }
+};
+
+// A row of at least 8 logits in slots of 8.  The last slot is read from V - 8:
+// what it repeats of the one before is taken as -inf.  NaN is let through: it
+// is not the larger of two, not at least anything, and weighs nothing.  Rows need not
+// be aligned (a 16-byte load at an element's alignment is legal here).  A pass
+// reads the row anew; after the first it comes from the L2.
 template <typename T> struct Row {
-  const T* p;      // the row
-  int V, off;      // off: elements from the 16-byte line that p lies in
-  static constexpr int N = 8;
-  // element e of slot q is logit q*8 + e - off, so that whole slots are aligned
-  DEVINL int index(int q, int e) const { return q * N + e - off; }
-  DEVINL int slots() const { return (V + off + N - 1) / N; }
-  DEVINL void load(int q, float* x) const {
-    const int i0 = q * N - off;
-    if (i0 >= 0 && i0 + N <= V) {
-      constexpr int W = 16 / sizeof(T);
+  const T* p;
+  int V;
+  bool only_inf;       // the maximum is +inf: those count as 0, others as -inf
+
+  DEVINL int slots() const { return (V + 7) / 8; }
+  DEVINL int first(int q) const { return min(q * 8, V - 8); }   // of slot q
+  DEVINL float at(int i) const {
+    const float x = DT<T>::to_f32(p[i]);
+    return !only_inf ? x : x == INFINITY ? 0.f : -INFINITY;
+  }
+  struct Raw { T v[8]; };
+  DEVINL Raw fetch(int q) const {
+    Raw r;
+    __builtin_memcpy(r.v, p + first(q), sizeof(r.v));
+    return r;
+  }
+  DEVINL f32x8 take8(const Raw& r, int q) const {
+    f32x8 x;
 #pragma unroll
-      for (int v = 0; v < N; v += W) {
-        const VecT<T, W> in = vload<T, W>(p + i0 + v);
+    for (int e = 0; e < 8; ++e) x[e] = DT<T>::to_f32(r.v[e]);
+    if (only_inf) {
 #pragma unroll
-        for (int u = 0; u < W; ++u) x[v + u] = DT<T>::to_f32(in.data[u]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        x[e] = i0 + e >= 0 && i0 + e < V ? DT<T>::to_f32(p[i0 + e]) : -INFINITY;
+      for (int e = 0; e < 8; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
     }
+    if (q * 8 > V - 8) {
+      const int skip = q * 8 - (V - 8);
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;   // NaN: not there
+      for (int e = 0; e < 8; ++e) x[e] = e < skip ? -INFINITY : x[e];
+    }
+    return x;
+  }
+  // f(8 logits, slot) for this thread's slots.  Every thread makes the same
+  // number of calls; slots from slots() on are -inf.  each4: a call is cheap,
+  // four slots are loaded at a time; each1: it is not, the next is on its way.
+  template <typename F> DEVINL void each4(F f) const {
+    const int n = (slots() + THREADS - 1) / THREADS;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 4) {
+      Raw r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = fetch(threadIdx.x + (i + j) * THREADS);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int q = threadIdx.x + (i + j) * THREADS;
+        f(take8(r[j], q), q);
+      }
+    }
+  }
+  template <typename F> DEVINL void each1(F f) const {
+    const int n = (slots() + THREADS - 1) / THREADS;
+    Raw next = fetch(threadIdx.x);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int q = threadIdx.x + i * THREADS;
+      const Raw r = next;
+      next = fetch(q + THREADS);
+      f(take8(r, q), q);
+    }
+  }
+  DEVINL unsigned bits_from(f32x8 x, float low) const {
+    unsigned bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits |= x[e] >= low && x[e] > -INFINITY ? 1u << e : 0u;
+    return bits;
+  }
+  // f(x, index) for the few elements that are at least `low`
+  template <typename F> DEVINL void each_from(float low, F f) const {
+    each1([&](f32x8 x, int q) {
+      unsigned bits = bits_from(x, low);
+#pragma unroll 1
+      while (bits) {
+        const int b = __builtin_ctz(bits);
+        bits &= bits - 1;
+        f(pick(x, b), first(q) + b);
+      }
+    });
+  }
+  static DEVINL float pick(f32x8 x, int b) {
+    float v = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) v = b == e ? x[e] : v;
+    return v;
   }
 };
 
-DEVINL u64 shfl_up64(u64 x, int d) { return __shfl_up(x, d, 64); }
-
-DEVINL u64 wave_sum64(u64 x) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off, 64);
+// Inclusive sum over the lanes, in six steps along the row (no LDS).
+template <int CTRL, int ROWS> DEVINL int moved(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> DEVINL u64 moved(u64 x) {
+  const unsigned lo = moved<CTRL, ROWS>((int)(unsigned)x);
+  const unsigned hi = moved<CTRL, ROWS>((int)(unsigned)(x >> 32));
+  return (u64)hi << 32 | lo;
+}
+template <typename I> DEVINL I wave_scan(I x) {
+  x += moved<0x111, 0xf>(x);             // from the lane 1, 2, 4, 8 before, in rows of 16
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);             // lane 15 of a row to the next row
+  x += moved<0x143, 0xc>(x);             // lane 31 to the upper half
   return x;
 }
-DEVINL u64 wave_scan64(u64 x) {          // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const u64 y = shfl_up64(x, off);
-    if (lane >= off) x += y;
-  }
-  return x;
+DEVINL u64 last_lane(u64 x) {
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)x, 63);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(x >> 32), 63);
+  return (u64)hi << 32 | lo;
 }
+DEVINL int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
+template <typename I> DEVINL I wave_sum(I x) { return last_lane(wave_scan(x)); }
 
 struct Shared {
-  u64 hist[BINS];
-  u64 cand_w[CAP];
-  u64 cand_k[CAP];
+  u64 hist[BINS];                        // and the logits of the last segment
+  u64 cand_k[CAP], cand_w[CAP], sum[CAP];
+  u64 list_k[LIST], list_w[LIST];
   u64 seg[SEGS];
   u64 wave_tot[WAVES];
-  double table[64];
-  float red[16];
-  u64 found_before, border;
-  int found_bin, cand_n;
+  u64 table[TABLE];
+  float red[2][WAVES];
+  u64 found_before, border, last_want;
+  int found_bin, cand_n, list_n, last_seg, greedy;
 };
 
-struct Weights {
-  float max;
-  double inv_t;
-  const double* table;
-  DEVINL u64 of(float x) const {
-    const double w = x == max ? 1.0 : exp_neg(((double)x - (double)max) * inv_t, table);
-    // w * 2^44 in the low bits of a double over 2^52: rounded to an integer
-    const double d = __builtin_fma(w, 17592186044416.0, 4503599627370496.0);
-    return __builtin_bit_cast(u64, d) & 0xfffffffffffffull;
-  }
-};
-
-// The first bin with whose elements the running sum reaches what a cut needs:
-// leaves it and what lies before it in s.found_*.  Every thread calls it.
-template <typename Reached>
-DEVINL void find_bin(Shared& s, Reached reached) {
+// The first bin with whose elements the running sum, from `outer`, reaches what
+// a cut needs: leaves it and what lies before it in s.found_*, or -1.
+// `need(total)` gives the cut's test for the sum over all, which is `total`, or
+// with 0 that of the histogram.  Every thread calls it, after a barrier behind
+// the histogram and with s.found_bin at -1; returns the total.
+template <typename Need> DEVINL u64 find_bin(Shared& s, u64 outer, u64 total, Need need) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const u64 a = s.hist[2 * t], b = s.hist[2 * t + 1];
-  const u64 inc = wave_scan64(a + b);
+  const u64 inc = wave_scan(a + b);
   if (lane == 63) s.wave_tot[wave] = inc;
   __syncthreads();
-  u64 before = inc - (a + b);
-  for (int w = 0; w < wave; ++w) before += s.wave_tot[w];
-  // exactly one thread finds its bin: the first to reach
-  if (!reached(before) && reached(before + a)) { s.found_bin = 2 * t; s.found_before = before; }
-  else if (!reached(before + a) && reached(before + a + b)) {
-    s.found_bin = 2 * t + 1;
-    s.found_before = before + a;
+  u64 before = outer + inc - (a + b), all = outer;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const u64 v = s.wave_tot[w];
+    before += w < wave ? v : 0;
+    all += v;
+  }
+  if (!total) total = all;
+  const auto reached = need(total);
+  // at most one thread has the first bin to reach
+  if (!reached(before) && reached(before + a + b)) {
+    const bool second = !reached(before + a);
+    s.found_bin = 2 * t + second;
+    s.found_before = second ? before + a : before;
+  }
+  __syncthreads();
+  return total;
+}
+
+// Empties the histogram and the candidates; barriers on both sides.
+DEVINL void clear(Shared& s) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) s.hist[i] = 0;
+  if (threadIdx.x == 0) { s.cand_n = 0; s.found_bin = -1; }
+  __syncthreads();
+}
+
+// s.sum[i] = the sum of of(i, j) over all j < n, for n <= CAP elements, in
+// integers of type I.  Where n is small, several waves share an element's sum.
+// Barriers on both sides.
+template <typename I, typename Of> DEVINL void pair_sums(Shared& s, int n, Of of) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (t < n) s.sum[t] = 0;
+  __syncthreads();
+  const int each = (n + 63) / 64;                  // waves for all elements once
+  const int parts = WAVES / max(each, 1), part = wave / max(each, 1);
+  const int i = (wave - part * each) * 64 + lane;
+  const int run = (n + parts - 1) / parts;
+  if (part < parts && i < n) {
+    I sum = 0;
+    const int end = min(n, (part + 1) * run);
+#pragma unroll 4
+    for (int j = part * run; j < end; ++j) sum += of(i, j);
+    if (sum) atomicAdd(&s.sum[i], (u64)sum);
   }
   __syncthreads();
 }
 
-// The border element: the last one, in the row's order, that a cut keeps.
-//   value(x): what an element adds to the running sum (1, or its weight);
-//   elements below floor_key do not count.
-//   reached(sum): whether a running sum is all that the cut keeps; false for 0,
-//   true for the sum over all.
-template <typename T, typename Value, typename Reached>
-DEVINL u64 find_border(Shared& s, const Row<T>& row, float max, float bin_scale, u64 floor_key,
-                       Value value, Reached reached) {
+// Among the n candidates the one with which the running sum, from `before`,
+// reaches.
+template <typename Reached> DEVINL u64 rank_candidates(Shared& s, int n, u64 before, Reached reached) {
   const int t = threadIdx.x;
-  const int slots = row.slots();
-  auto bin_of = [&](float x) {
-    const float d = x == max ? 0.f : max - x;
-    return (int)fminf(d * bin_scale, (float)(BINS - 1));
-  };
-  for (int i = t; i < BINS; i += THREADS) s.hist[i] = 0;
-  if (t == 0) s.cand_n = 0;
-  __syncthreads();
-  for (int q = t; q < slots; q += THREADS) {
-    float x[8];
-    row.load(q, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (x[e] > -INFINITY && rank_key(x[e], row.index(q, e)) >= floor_key)
-        atomicAdd(&s.hist[bin_of(x[e])], value(x[e]));
+  pair_sums<u64>(s, n, [&](int i, int j) { return s.cand_k[j] > s.cand_k[i] ? s.cand_w[j] : 0; });
+  if (t < n) {
+    const u64 sum = before + s.sum[t];
+    if (!reached(sum) && reached(sum + s.cand_w[t])) s.border = s.cand_k[t];
   }
   __syncthreads();
-  find_bin(s, reached);
-  const int bin = s.found_bin;
-  u64 before = s.found_before;
-  // the bin's elements, if they fit
-  for (int q = t; q < slots; q += THREADS) {
-    float x[8];
-    row.load(q, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (x[e] > -INFINITY && bin_of(x[e]) == bin) {
-        const u64 k = rank_key(x[e], row.index(q, e));
-        if (k >= floor_key) {
-          const int at = atomicAdd(&s.cand_n, 1);
-          if (at < CAP) { s.cand_k[at] = k; s.cand_w[at] = value(x[e]); }
-        }
-      }
-  }
-  __syncthreads();
-  const int n = s.cand_n;
-  if (n <= CAP) {
-    if (t < n) {
-      const u64 mine = s.cand_k[t];
-      u64 sum = before;
-      for (int j = 0; j < n; ++j) sum += s.cand_k[j] > mine ? s.cand_w[j] : 0;
-      if (!reached(sum) && reached(sum + s.cand_w[t])) s.border = mine;
-    }
-    __syncthreads();
-    return s.border;
-  }
-  // Too many share the bin (a flat row, or masks of a finite value stretched
-  // it): narrow the border down by 11 bits of the order's key at a time.
-  u64 prefix = 0;
-  int shift = 64;
-  while (shift > 0) {
-    const int bits = min(11, shift);
-    const int up = shift;
-    shift -= bits;
-    __syncthreads();
-    for (int i = t; i < BINS; i += THREADS) s.hist[i] = 0;
-    __syncthreads();
-    for (int q = t; q < slots; q += THREADS) {
-      float x[8];
-      row.load(q, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!(x[e] > -INFINITY) || bin_of(x[e]) != bin) continue;
-        const u64 k = rank_key(x[e], row.index(q, e));
-        if (k < floor_key || (up < 64 && (k >> up) != prefix)) continue;
-        // bin 0 holds the largest
-        const int b = (1 << bits) - 1 - (int)(k >> shift & ((1u << bits) - 1));
-        atomicAdd(&s.hist[b], value(x[e]));
-      }
-    }
-    __syncthreads();
-    const u64 outer = before;
-    find_bin(s, [&](u64 sum) { return reached(outer + sum); });
-    before = outer + s.found_before;
-    prefix = prefix << bits | (u64)((1 << bits) - 1 - s.found_bin);
-  }
-  return prefix;
+  return s.border;
 }
 
-template <typename T, typename U>
-__global__ void __launch_bounds__(THREADS)
-sample_kernel(const T* __restrict__ logits, long ld, int V, const U* __restrict__ uniform,
-              Opt temperature, Opt top_k, Opt top_p, Opt min_p, long empty_token,
-              long* __restrict__ out) {
-  __shared__ Shared s;
-  const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  Row<T> row;
-  row.p = logits + r * ld;
-  row.V = V;
-  row.off = (int)(reinterpret_cast<uintptr_t>(row.p) % 16 / sizeof(T));
-  const int slots = row.slots();
-  if (t < 64) s.table[t] = EXP2_64[t];
+// A running sum of integers is over u * total exactly if it is over this one;
+// the last one always is.
+DEVINL u64 last_before(double u, u64 total) {
+  const double target = u * (double)total;
+  const u64 want = target > 0.0 ? (u64)target : 0;
+  return want < total ? want : total - 1;
+}
 
-  // extremes of what is there
-  float mx = -INFINITY, mn = INFINITY, there = 0.f;
-  for (int q = t; q < slots; q += THREADS) {
-    float x[8];
-    row.load(q, x);
+DEVINL void candidate(Shared& s, u64 key, u64 w) {
+  const int to = atomicAdd(&s.cand_n, 1);
+  if (to < CAP) { s.cand_k[to] = key; s.cand_w[to] = w; }
+}
+
+// All elements of at least `low` to the list, as far as it goes.  Where a
+// wave's logit goes follows from masks in scalar registers: a logit that no
+// lane lists costs a comparison.
+template <typename T> DEVINL void list_from(Shared& s, const Row<T>& row, float low) {
+  const int lane = threadIdx.x & 63;
+  low = fmaxf(low, -3.402823466e38f);
+  row.each4([&](f32x8 x, int q) {
+    u64 who[8];
+    int all = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      mx = fmaxf(mx, x[e]);
-      mn = fminf(mn, x[e] > -INFINITY ? x[e] : INFINITY);
-      there += x[e] > -INFINITY ? 1.f : 0.f;
+      who[e] = __ballot(x[e] >= low);
+      all += __popcll(who[e]);
     }
+    if (!all) return;
+    int to = 0;
+    if (lane == 0) to = atomicAdd(&s.list_n, all);
+    to = __builtin_amdgcn_readfirstlane(to);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (!who[e]) continue;
+      const int at = to + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who[e] >> 32),
+                                                         __builtin_amdgcn_mbcnt_lo((unsigned)who[e], 0));
+      if (x[e] >= low && at < LIST) s.list_k[at] = rank_key(x[e], row.first(q) + e);
+      to += __popcll(who[e]);
+    }
+  });
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restrict__ uniform,
+              bool uniform_is_double, Opt temperature, Opt top_k, Opt top_p, Opt min_p,
+              long empty_token, long* __restrict__ out) {
+  __shared__ Shared s;
+  const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  Row<T> row{logits + r * ld, V, false};
+
+  // this thread's largest, the row's, and the smallest of the threads'
+  float mine = -INFINITY;
+  row.each4([&](f32x8 x, int) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine = fmaxf(mine, x[e]);
+  });
+  if (t < TABLE) s.table[t] = EXP2_TABLE[t];
+  for (int i = t; i < BINS; i += THREADS) s.hist[i] = 0;
+  if (t == 0) { s.cand_n = s.list_n = 0; s.found_bin = -1; s.greedy = 0x7fffffff; }
+  float mx = wave_reduce_max(mine);
+  float mn = -wave_reduce_max(mine > -INFINITY ? -mine : -INFINITY);
+  if (lane == 0) { s.red[0][wave] = mx; s.red[1][wave] = mn; }
+  double temp = temperature.f(r);
+  const int k = top_k.i(r);
+  const double p = top_p.f(r);
+  double floor_p = min_p.f(r);
+  const double u = uniform_is_double ? ((const double*)uniform)[r] : ((const float*)uniform)[r];
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    mx = fmaxf(mx, s.red[0][w]);
+    mn = fminf(mn, s.red[1][w]);
   }
-  mx = block_reduce_max(mx, s.red);
-  mn = -block_reduce_max(-mn, s.red);
-  there = block_reduce_sum(there, s.red);          // exact: under 2^24
   if (mx == -INFINITY) {
     if (t == 0) out[r] = empty_token;
     return;
   }
-
-  double temp = temperature.f(r);
-  int k = top_k.i(r);
-  const double p = top_p.f(r);
-  double floor_w = min_p.f(r);
-  if (!(temp > 0.0)) { temp = 1.0; k = 1; }
-  floor_w = floor_w < 1.0 ? floor_w : 1.0;       // the maximum always stays
-  const Weights w{mx, 1.0 / temp, s.table};
-  const u64 min_w = floor_w > 0.0 ? (u64)ceil(floor_w * 17592186044416.0 - 0.5) : 0;
-
-  // bins over the distance from the maximum that matters; what is further
-  // shares the last one
-  const float range = fminf(mx - mn, 64.f * fmaxf(1.f, (float)temp));
-  const float bin_scale = range > 0.f ? fminf((float)(BINS - 1) / range, 1e30f) : 0.f;
-
-  u64 border = NO_BORDER;
-  if (k > 0 && k < V) {
-    // fewer than k may be there: then all stay
-    const u64 need = k;
-    if (there > (float)k)
-      border = find_border(s, row, mx, bin_scale, NO_BORDER, [](float) { return (u64)1; },
-                           [&](u64 sum) { return sum >= need; });
+  if (mx == INFINITY) {
+    row.only_inf = true;
+    mx = mn = 0.f;
   }
-  __syncthreads();
-  if (p < 1.0 && k != 1) {
-    // the sum over K first
-    u64 mine = 0;
-    for (int q = t; q < slots; q += THREADS) {
-      float x[8];
-      row.load(q, x);
+  if (!(temp > 0.0) || k == 1 || p <= 0.0) {        // the first of the order
+    row.each_from(mx, [&](float, int idx) { atomicMin(&s.greedy, idx); });
+    __syncthreads();
+    if (t == 0) out[r] = s.greedy;
+    return;
+  }
+
+  const double slope = 46.16624130844683 / temp;
+  // 48 * 32 / slope below the maximum, or a rounding of it: over 2^-46.5 away
+  const Weights weight{(double)mx, slope, mx - (float)(48.0 * TABLE / slope), s.table};
+  floor_p = floor_p < 1.0 ? floor_p : 1.0;          // the maximum always stays
+  const u64 min_w = floor_p > 0.0 ? (u64)__builtin_rint(floor_p * ONE) : 0;
+
+  // Bins over the distance from the maximum that matters: the spread of the
+  // threads' largest, which a few masked logits do not stretch, or three times
+  // it; what is further shares the last bin.  Rounding keeps the order: a bin
+  // holds a run of it.
+  const float range = fminf(mx - mn, 64.f * fmaxf(1.f, (float)temp));
+  const float narrow = range > 0.f ? fminf((float)(BINS - 2) / range, 1e30f) : 0.f;
+  float bin_scale = narrow;
+  auto bin_of = [&](float x) {
+    return (int)fminf((mx - x) * bin_scale, (float)(BINS - 1));
+  };
+  // a value that is not above any of bins 0..b: one bin more, for its roundings
+  auto low_of = [&](int b) {
+    return b >= BINS - 2 || !(bin_scale > 0.f) ? -INFINITY : mx - (float)(b + 2) / bin_scale;
+  };
+
+  u64 border = 0;                                   // the last element kept; 0: all are
+  bool ordered = false;                             // and top-p is done
+  bool listed = false;                              // the list holds all up to the border
+
+  // Leaves border, and the list where what is not behind `bin` fits (all that
+  // the cut keeps, and a few more).  Of `bin`, what is not below floor_key and
+  // reached() keeps stays.  value(x): what an element adds to the running sum,
+  // which is `before` where the bin begins.
+  auto cut_in_bin = [&](int bin, u64 before, u64 floor_key, auto value, auto reached) {
+    list_from(s, row, low_of(bin));
+    listed = s.list_n <= LIST;
+    if (listed) {
+      const int n = s.list_n;
+      for (int i = t; i < n; i += THREADS) {
+        const u64 key = s.list_k[i];
+        const float x = value_of(key);
+        s.list_w[i] = weight.of(x);
+        if (bin_of(x) == bin && key >= floor_key) candidate(s, key, value(x));
+      }
+    } else {
+      row.each_from(low_of(bin), [&](float x, int idx) {
+        const u64 key = rank_key(x, idx);
+        if (bin_of(x) == bin && key >= floor_key) candidate(s, key, value(x));
+      });
+    }
+    __syncthreads();
+    const int n = s.cand_n;
+    if (n <= CAP) {
+      border = rank_candidates(s, n, before, reached);
+      return;
+    }
+    // Too many share the bin (a flat row, or few distinct values): narrow the
+    // border down by 11 bits of the key at a time.
+    u64 prefix = 0;
+#pragma unroll 1
+    for (int shift = 64; shift > 0;) {
+      const int up = shift, bits = min(11, shift);
+      shift -= bits;
+      clear(s);
+      row.each_from(low_of(bin), [&](float x, int idx) {
+        const u64 key = rank_key(x, idx);
+        if (bin_of(x) != bin || key < floor_key || (up < 64 && (key >> up) != prefix)) return;
+        // bin 0 holds the largest
+        atomicAdd(&s.hist[(1 << bits) - 1 - (int)(key >> shift & ((1u << bits) - 1))], value(x));
+      });
+      __syncthreads();
+      find_bin(s, before, 0, [&](u64) { return reached; });
+      before = s.found_before;
+      prefix = prefix << bits | (u64)((1 << bits) - 1 - s.found_bin);
+    }
+    border = prefix;
+  };
+
+  if (k > 0 && k < V) {
+    const u64 want = k;
+    const auto reached = [want](u64 sum) { return sum >= want; };
+    bool done = false;
+    if (k <= FEW) {
+      // The k-th largest of the threads' largest is a lower bound of the k-th
+      // largest: bins behind its own hold nothing of the first k.
+      if (mine > -INFINITY && !row.only_inf) atomicAdd(&s.hist[bin_of(mine)], (u64)1);
+      __syncthreads();
+      find_bin(s, 0, 0, [&](u64) { return reached; });
+      // fewer than k threads may hold anything: then no bound
+      const int bin = s.found_bin < 0 ? BINS - 1 : s.found_bin;
+      list_from(s, row, low_of(bin));
+      const int found = s.list_n;
+      if (found <= CAP) {
+        // the first k of them in the row's order, and their weights
+        pair_sums<int>(s, found, [&](int i, int j) { return (int)(s.list_k[j] > s.list_k[i]); });
+        const int n = min(found, k);
+        const u64 key = t < found ? s.list_k[t] : 0;
+        __syncthreads();
+        if (t < found && s.sum[t] < (u64)k) {
+          s.list_k[s.sum[t]] = key;
+          s.list_w[s.sum[t]] = weight.of(value_of(key));
+        }
+        if (t == 0) s.list_n = n;
+        __syncthreads();
+        if (n <= 64) {
+          // one wave, an element a lane, in the row's order
+          if (wave != 0) return;
+          u64 w = lane < n ? s.list_w[lane] : 0;
+          const int idx = lane < n ? index_of(s.list_k[lane]) : 0x7fffffff;
+          u64 end = wave_scan(w);
+          if (p < 1.0 && lane > 0 && (double)(end - w) >= p * (double)last_lane(end)) w = 0;
+          if (w < min_w) w = 0;
+          end = wave_scan(w);
+          const u64 last = last_before(u, last_lane(end));
+          u64 before = 0;                           // of lower index
+          for (int j = 0; j < n; ++j) {
+            const u64 lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)w, j);
+            const u64 hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(w >> 32), j);
+            before += __builtin_amdgcn_readlane(idx, j) < idx ? hi << 32 | lo : 0;
+          }
+          if (before <= last && before + w > last) out[r] = idx;
+          return;
+        }
+        if (wave == 0 && p < 1.0) {
+          // the next cut, from running sums in that order
+          constexpr int PER = FEW / 64;
+          u64 w[PER], own = 0;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            w[j] = lane * PER + j < n ? s.list_w[lane * PER + j] : 0;
+            own += w[j];
+          }
+          const u64 end = wave_scan(own);
+          const double enough = p * (double)last_lane(end);
+          u64 before = end - own;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int i = lane * PER + j;
+            if (i > 0 && i < n && (double)before >= enough) s.list_w[i] = 0;
+            before += w[j];
+          }
+        }
+        listed = done = ordered = true;
+      }
+      if (!done) {
+      clear(s);
+      if (t == 0) s.list_n = 0;
+      }
+    }
+    if (!done) {
+    bin_scale = narrow / 3;
+    row.each4([&](f32x8 x, int) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (x[e] > -INFINITY && rank_key(x[e], row.index(q, e)) >= border) mine += w.of(x[e]);
+        if (x[e] > -INFINITY) atomicAdd(&s.hist[bin_of(x[e])], (u64)1);
+    });
+    __syncthreads();
+    find_bin(s, 0, 0, [&](u64) { return reached; });
+    // fewer than k may be there: then all stay
+    if (s.found_bin >= 0)
+      cut_in_bin(s.found_bin, s.found_before, 0, [](float) { return (u64)1; }, reached);
     }
-    mine = wave_sum64(mine);
-    if (lane == 0) s.wave_tot[wave] = mine;
-    __syncthreads();
-    u64 total = 0;
-    for (int v = 0; v < WAVES; ++v) total += s.wave_tot[v];
-    __syncthreads();
-    const double need = p * (double)total;
-    // sum > 0: at least the first stays
-    border = find_border(s, row, mx, bin_scale, border, [&](float x) { return w.of(x); },
-                         [&](u64 sum) { return sum > 0 && (double)sum >= need; });
   }
-  __syncthreads();
 
-  // kept weights in index order: a sum for each wave's 512 logits
+  if (p < 1.0 && !ordered) {
+    const auto need = [p](u64 total) {
+      const double enough = p * (double)total;
+      return [enough](u64 sum) { return sum > 0 && (double)sum >= enough; };
+    };
+    clear(s);
+    if (listed) {
+      const int n = s.list_n;
+      for (int i = t; i < n; i += THREADS) {
+        if (s.list_k[i] < border) s.list_w[i] = 0;  // behind the first k
+        atomicAdd(&s.hist[bin_of(value_of(s.list_k[i]))], s.list_w[i]);
+      }
+      __syncthreads();
+      const auto reached = need(find_bin(s, 0, 0, need));
+      const int bin = s.found_bin;
+      const u64 before = s.found_before;
+      for (int i = t; i < n; i += THREADS)
+        if (bin_of(value_of(s.list_k[i])) == bin) candidate(s, s.list_k[i], s.list_w[i]);
+      __syncthreads();
+      if (s.cand_n <= CAP) {
+        border = rank_candidates(s, s.cand_n, before, reached);
+      } else {
+        // rank them against the list itself, a few for each thread
+        for (int i = t; i < n; i += THREADS) {
+          const u64 key = s.list_k[i];
+          if (bin_of(value_of(key)) != bin) continue;
+          u64 sum = 0;
+          for (int j = 0; j < n; ++j) sum += s.list_k[j] > key ? s.list_w[j] : 0;
+          if (!reached(sum) && reached(sum + s.list_w[i])) s.border = key;
+        }
+        __syncthreads();
+        border = s.border;
+      }
+    } else {
+      const u64 floor_key = border;
+      bin_scale = narrow;
+      if (t == 0) s.list_n = 0;
+      // Only what is at least every thread's largest goes to the histogram at
+      // first: the border is hardly ever below, and the atomics cost as much
+      // as the weights.
+      u64 total = 0;
+      auto weigh = [&](auto floored) {
+        row.each1([&](f32x8 x, int q) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            u64 w = weight.of(x[e]);
+            if (floored && rank_key(x[e], row.first(q) + e) < floor_key) w = 0;
+            total += w;
+            if (x[e] >= mn) atomicAdd(&s.hist[bin_of(x[e])], w);
+          }
+        });
+      };
+      if (floor_key) weigh(std::true_type());
+      else weigh(std::false_type());
+      total = wave_sum(total);
+      if (lane == 0) s.cand_w[wave] = total;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) total += s.cand_w[w];
+      find_bin(s, 0, total, need);
+      if (s.found_bin < 0) {
+        clear(s);
+        bin_scale = narrow / 3;
+        row.each1([&](f32x8 x, int q) {
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) {
+            const float v = Row<T>::pick(x, e);
+            if (v > -INFINITY && (!floor_key || rank_key(v, row.first(q) + e) >= floor_key))
+              atomicAdd(&s.hist[bin_of(v)], weight.of(v));
+          }
+        });
+        __syncthreads();
+        find_bin(s, 0, total, need);
+      }
+      cut_in_bin(s.found_bin, s.found_before, floor_key,
+                 [&](float x) { return weight.of(x); }, need(total));
+    }
+  }
+
+  // A short list: the running sum in index order, each element for itself.
+  __syncthreads();
+  if (listed && s.list_n <= SHORT) {
+    const int n = s.list_n;
+    u64 w = 0;
+    if (t < n) {
+      w = s.list_k[t] >= border && s.list_w[t] >= min_w ? s.list_w[t] : 0;
+      s.list_w[t] = w;
+    }
+    __syncthreads();
+    // keys of an index hold its complement
+    pair_sums<u64>(s, n, [&](int i, int j) {
+      return (unsigned)s.list_k[j] >= (unsigned)s.list_k[i] ? s.list_w[j] : 0;
+    });
+    u64 total = 0;                                  // the largest of the running sums
+    if (wave == 0) {
+      for (int i = lane; i < n; i += 64) total += s.list_w[i];
+      total = wave_sum(total);
+      if (lane == 0) s.last_want = last_before(u, total);
+    }
+    __syncthreads();
+    if (t < n && s.sum[t] > s.last_want && s.sum[t] - w <= s.last_want) out[r] = index_of(s.list_k[t]);
+    return;
+  }
+
+  // Kept weights in index order: a sum for each segment of 512, the segment
+  // that the number falls into, and the logit in it.
+  const int nseg = (V + SEG - 1) / SEG;
+  __syncthreads();
+  for (int i = t; i < nseg; i += THREADS) s.seg[i] = 0;
+  for (int i = t; i < SEG; i += THREADS) s.hist[i] = 0;
   auto kept = [&](float x, int idx) -> u64 {
-    if (!(x > -INFINITY) || rank_key(x, idx) < border) return 0;
-    const u64 v = w.of(x);
+    const u64 v = x > -INFINITY && rank_key(x, idx) >= border ? weight.of(x) : 0;
     return v >= min_w ? v : 0;
   };
-  const int nseg = (slots + 63) / 64;
-  for (int q = t; q < nseg * 64; q += THREADS) {
-    u64 mine = 0;
-    if (q < slots) {
-      float x[8];
-      row.load(q, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mine += kept(x[e], row.index(q, e));
+  __syncthreads();
+  const int n_list = s.list_n;
+  if (listed) {
+    for (int i = t; i < n_list; i += THREADS) {
+      const u64 v = s.list_k[i] >= border && s.list_w[i] >= min_w ? s.list_w[i] : 0;
+      s.list_w[i] = v;
+      if (v) atomicAdd(&s.seg[index_of(s.list_k[i]) / SEG], v);
     }
-    mine = wave_sum64(mine);
-    if (lane == 0) s.seg[q >> 6] = mine;
+  } else {
+    row.each1([&](f32x8 x, int q) {
+      u64 sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += kept(x[e], row.first(q) + e);
+      sum = wave_sum(sum);
+      if (lane == 0 && (q >> 6) < nseg) s.seg[q >> 6] = sum;
+    });
   }
   __syncthreads();
-  if (wave != 0) return;
-  u64 own = 0;                               // lane's run of segments
-  const int per = (nseg + 63) / 64;
-  for (int i = 0; i < per; ++i)
-    if (lane * per + i < nseg) own += s.seg[lane * per + i];
-  const u64 inc = wave_scan64(own);
-  const u64 total = __shfl(inc, 63, 64);
-  const double target = (double)uniform[r] * (double)total;
-  u64 want = target > 0.0 ? (u64)target : 0;  // running sum > u*total, in integers
-  if (want >= total) want = total - 1;
-  const u64 hits = __ballot(inc > want);
-  const int owner = __ffsll(hits) - 1;
-  int seg = 0;
-  u64 before = inc - own;
-  if (lane == owner)
-    for (int i = 0; i < per; ++i) {
-      const u64 v = lane * per + i < nseg ? s.seg[lane * per + i] : 0;
-      seg = lane * per + i;
-      if (before + v > want) break;
-      before += v;
+  if (wave == 0) {
+    const int per = (nseg + 63) / 64;               // a lane's run of segments
+    const int from = min(lane * per, nseg), upto = min(from + per, nseg);
+    u64 own = 0;
+    for (int i = from; i < upto; ++i) own += s.seg[i];
+    const u64 end = wave_scan(own);
+    const u64 total = last_lane(end);
+    const u64 want = last_before(u, total);
+    u64 before = end - own;
+    if (before <= want && end > want) {
+      int i = from;
+      while (before + s.seg[i] <= want) before += s.seg[i++];
+      s.last_seg = i;
+      s.last_want = want - before;                  // what is left inside it
     }
-  seg = __shfl(seg, owner, 64);
-  before = __shfl(before, owner, 64);
-  const int q = seg * 64 + lane;
-  float x[8];
-  u64 kw[8], sum = 0;
-  if (q < slots) row.load(q, x);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    kw[e] = q < slots ? kept(x[e], row.index(q, e)) : 0;
-    sum += kw[e];
   }
-  const u64 upto = wave_scan64(sum) + before;
-  const int who = __ffsll(__ballot(upto > want)) - 1;
-  if (lane == who) {
-    u64 c = upto - sum;
-    int id = 0;
-    bool done = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      c += kw[e];
-      if (!done && c > want) { id = row.index(q, e); done = true; }
+  __syncthreads();
+  const int seg = s.last_seg;
+  if (listed) {
+    for (int i = t; i < n_list; i += THREADS) {
+      const int at = index_of(s.list_k[i]);
+      if (at / SEG == seg) s.hist[at % SEG] = s.list_w[i];
     }
-    out[r] = id;
+  } else if (t < SEG && seg * SEG + t < V) {
+    s.hist[t] = kept(row.at(seg * SEG + t), seg * SEG + t);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    u64 w[8], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { w[e] = s.hist[lane * 8 + e]; sum += w[e]; }
+    const u64 want = s.last_want, end = wave_scan(sum);
+    if (end - sum <= want && end > want) {
+      u64 c = end - sum;
+      int e = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c += w[j];
+        e += c <= want;
+      }
+      out[r] = seg * SEG + lane * 8 + e;
+    }
   }
 }
 
@@ -440,22 +767,18 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
   c10::DeviceGuard guard(logits.device());
   auto out = torch::empty({B}, logits.options().dtype(torch::kLong));
   if (B == 0) return out;
+  if (V < 8) logits = at::constant_pad_nd(logits, {0, 8 - V}, -INFINITY);   // a slot at least
   if (logits.stride(1) != 1) logits = logits.contiguous();
   auto stream = at::hip::getCurrentHIPStream().stream();
-#define SAMPLE(T, U)                                                                               \
-  hipLaunchKernelGGL((sample_kernel<T, U>), dim3(B), dim3(THREADS), 0, stream,                     \
-                     (const T*)logits.data_ptr(), (long)logits.stride(0), (int)V,                  \
-                     (const U*)u.data_ptr(), ot, ok, op, om, empty_token, out.data_ptr<long>())
-#define BY_U(T)                                                 \
-  do {                                                          \
-    if (u.scalar_type() == torch::kFloat) SAMPLE(T, float);     \
-    else SAMPLE(T, double);                                     \
-  } while (0)
-  if (logits.scalar_type() == torch::kBFloat16) BY_U(__hip_bfloat16);
-  else if (logits.scalar_type() == torch::kHalf) BY_U(__half);
-  else if (logits.scalar_type() == torch::kFloat) BY_U(float);
+  const bool is_double = u.scalar_type() == torch::kDouble;
+#define SAMPLE(T)                                                                                 \
+  hipLaunchKernelGGL((sample_kernel<T>), dim3(B), dim3(THREADS), 0, stream,                        \
+                     (const T*)logits.data_ptr(), (long)logits.stride(0), (int)logits.size(1), u.data_ptr(),    \
+                     is_double, ot, ok, op, om, empty_token, out.data_ptr<long>())
+  if (logits.scalar_type() == torch::kBFloat16) SAMPLE(__hip_bfloat16);
+  else if (logits.scalar_type() == torch::kHalf) SAMPLE(__half);
+  else if (logits.scalar_type() == torch::kFloat) SAMPLE(float);
   else TORCH_CHECK(false, "sample_tokens: bf16, fp16 or fp32 logits, got ", logits.scalar_type());
-#undef BY_U
 #undef SAMPLE
   HIP_CHECK_KERNEL();
   return out;
