@@ -21,7 +21,9 @@
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
@@ -191,6 +193,76 @@ kv8_append_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, Str3 k
   if (threadIdx.x == 0) *scale_at = scale;
 }
 
+// four codes at another scale: `ratio` is a power of two of at most 1
+DEVINL unsigned rescale4(unsigned codes, float ratio) {
+  float o[4];
+  decode4(codes, o);
+  return encode4(o[0] * ratio, o[1] * ratio, o[2] * ratio, o[3] * ratio);
+}
+
+// ---------------------------------------------------------------------------
+// Append of one token, a wave for a (sequence, head) of K or of V: a load, a
+// reduction over the wave and a byte a lane to store.  The codes of the block
+// are touched only if its scale has to grow, which happens to few tokens.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, Str3 kst, Str3 vst,
+                      unsigned char* __restrict__ kc, unsigned char* __restrict__ vc,
+                      float* __restrict__ ks, float* __restrict__ vs, PerSeq start, PerSeq counts,
+                      int BH, int H, int NB) {
+  constexpr int PER = D > 64 ? D / 64 : 1;        // values a lane holds
+  const int lane = threadIdx.x & 63;
+  const int bh = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const bool is_v = blockIdx.y;
+  if (bh >= BH) return;
+  const int b = bh / H, h = bh % H;
+  const int st = start.at(b);
+  if (st < 0 || st / BLK >= NB || counts.at(b) <= 0) return;
+  const int at = st % BLK;
+  const long blk = (long)bh * NB + st / BLK;
+  const T* src = is_v ? vnew + b * vst.b + h * vst.h : knew + b * kst.b + h * kst.h;
+  unsigned char* codes = (is_v ? vc : kc) + blk * (BLK * D);
+  float* scale_at = (is_v ? vs : ks) + blk;
+  const float old = at > 0 ? *scale_at : 0.f;
+  const int d0 = lane * PER;
+  float x[PER];
+  float amax = 0.f;
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    x[u] = d0 + u < D ? DT<T>::to_f32(src[d0 + u]) : 0.f;
+    amax = fmaxf(amax, finite_abs(x[u]));
+  }
+  const float scale = fmaxf(scale_for(wave_reduce_max(amax)), old);
+  const float inv = 1.f / scale;                  // exact: a power of two
+  if (at > 0 && scale > old) {
+    const float ratio = old * inv;
+    if (!is_v) {
+      for (int i = lane * 4; i < at * D; i += 256) {
+        unsigned* c = reinterpret_cast<unsigned*>(codes + i);
+        *c = rescale4(*c, ratio);
+      }
+    } else {
+      for (int i = lane; i < D * (BLK / 4); i += 64) {
+        const int t0 = i % (BLK / 4) * 4;
+        if (t0 >= at) continue;
+        unsigned* c = reinterpret_cast<unsigned*>(codes + i / (BLK / 4) * BLK + t0);
+        // codes behind the new token stay as they were
+        const unsigned mask = at - t0 >= 4 ? 0xffffffffu : (1u << (8 * (at - t0))) - 1u;
+        *c = (rescale4(*c, ratio) & mask) | (*c & ~mask);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    if (d0 + u >= D) break;
+    const unsigned char c = encode1(x[u] * inv);
+    if (is_v) codes[(d0 + u) * BLK + at] = c;
+    else codes[at * D + d0 + u] = c;
+  }
+  if (lane == 0) *scale_at = scale;
+}
+
 // ---------------------------------------------------------------------------
 // Attention of one query token over the cache.
 //
@@ -203,10 +275,18 @@ kv8_append_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, Str3 k
 // the query's type and the block's scale is multiplied into the score; V codes
 // are converted to bf16 with the scale applied by the conversion (exact).
 //
+// A group has GP = 1, 2, 4, 8 or 16 query heads (the next power of two) for the
+// matrix instruction's 16 columns.  Column c takes head c % GP and, of each
+// lane group's 16 tokens, the GP from c / GP * GP on: its other weights are 0,
+// and the columns of a head are summed at the end.  So a lane makes GP weights,
+// not 16, and a token's weight is made once.
+//
 // P is split into two bf16 numbers, p = hi + lo (16 significant bits, so P
-// adds no error beside the output's own rounding).  With at most 8 query heads
-// a group, columns 8..15 repeat the queries of 0..7 and carry `lo`: the same
-// instruction does both.  Scores, statistics and sums are fp32.
+// adds no error beside the output's own rounding).  The reference m that is
+// subtracted in the exponent is raised, and what was summed rescaled, only when
+// a score is over it by more than 8: weights then stay under e^8, which costs
+// no precision in fp32 and bf16, and most blocks do without a reduction over
+// the wave.  Scores, statistics and sums are fp32.
 //
 // Few rows and a long cache: the blocks of a sequence are dealt to `nsplit`
 // workgroups, whose (o, m, l) a second kernel joins.
@@ -265,28 +345,27 @@ struct AttnArgs {
   const float* kpad;   // (B, width) or null
   long bias_b, bias_h, kpad_b;
   float scale;
-  int Hq, H, G, NB, max_len, nsplit;
-  bool mask16;         // mask rows are 16-byte aligned
+  int BH, Hq, H, G, NB, max_len, nsplit;
+  int share;           // waves that share a sequence and head: 1, 2 or 4 of a workgroup's 4
 };
 
+constexpr int MAX_SPLIT = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// sixteen values of a mask row from token tok0; behind the sequence's end the
-// last one again
-DEVINL void mask16(const float* row, int tok0, int len, bool aligned, f32x4* out) {
-  if (aligned && tok0 + 16 <= len) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) out[t] = *reinterpret_cast<const f32x4*>(row + tok0 + 4 * t);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[t][r] = row[min(tok0 + 4 * t + r, len - 1)];
-  }
+// op over the columns of a head: lanes of a row of 16 that are GP apart
+template <int GP, typename Op> DEVINL float over_columns(float x, Op op) {
+  auto turned = [](float v, auto by) {            // from the lane `by` on, round the row
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+        0, __builtin_bit_cast(int, v), 0x120 + by, 0xf, 0xf, false));
+  };
+  if (GP < 16) x = op(x, turned(x, std::integral_constant<int, 8>()));
+  if (GP < 8) x = op(x, turned(x, std::integral_constant<int, 4>()));
+  if (GP < 4) x = op(x, turned(x, std::integral_constant<int, 2>()));
+  if (GP < 2) x = op(x, turned(x, std::integral_constant<int, 1>()));
+  return x;
 }
 
-// WIDE: more than 8 query heads a cache head
-template <typename T, int D, bool WIDE, bool BIAS, bool KPAD>
+template <typename T, int D, int GP>
 __global__ void __launch_bounds__(256)
 kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char* __restrict__ kc,
                 const unsigned char* __restrict__ vc, const float* __restrict__ ksc,
@@ -295,19 +374,22 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
   constexpr int WAVES = 4;
   constexpr int KSTEP = D / 32;        // matrix instructions along d
   constexpr int DT16 = D / 16;         // tiles of 16 d
-  constexpr int COLS = WIDE ? 16 : 8;  // query heads a workgroup takes
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
-  const long bh = blockIdx.x;
+  const int sub = wave & (a.share - 1);                // of the waves that share
+  const long bh_at = (long)blockIdx.x * (WAVES / a.share) + wave / a.share;
+  const bool there = bh_at < a.BH;
+  const long bh = there ? bh_at : 0;
   const int b = bh / a.H, h = bh % a.H;
   const int split = blockIdx.y;
-  const int q0 = blockIdx.z * COLS;                    // first query head of the group
-  const int col = WIDE ? c16 : (c16 & 7);
-  const bool lo_half = !WIDE && c16 >= 8;
+  const int q0 = blockIdx.z * GP;                      // first query head of the group
+  const int col = c16 % GP, part16 = c16 / GP;         // this lane's head, and its tokens
   const bool col_ok = q0 + col < a.G;
   const int hq = h * a.G + q0 + (col_ok ? col : 0);
   const int len = min(max(lengths.at(b), 0), a.max_len);
-  const int nblk = (len + BLK - 1) / BLK;
+  const int nblk = there ? (len + BLK - 1) / BLK : 0;
+  const float* bias = a.bias ? a.bias + b * a.bias_b + hq * a.bias_h : nullptr;
+  const float* kpad = a.kpad ? a.kpad + b * a.kpad_b : nullptr;
 
   // queries: lane (column, g) holds d = g*(D/4) + 8s + j
   typename KFrag<T>::vec qf[KSTEP];
@@ -321,10 +403,10 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
   f32x4 acc[DT16];
 #pragma unroll
   for (int i = 0; i < DT16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;       // l: this lane group's share
+  float m = -INFINITY, l = 0.f;       // m: of the head; l: this lane's share
 
   const int krow = (c16 >> 2) * 16 + (c16 & 3);
-  for (int blk = split * WAVES + wave; blk < nblk; blk += a.nsplit * WAVES) {
+  for (int blk = split * a.share + sub; blk < nblk; blk += a.nsplit * a.share) {
     const unsigned char* kb = kc + (bh * a.NB + blk) * (long)(BLK * D);
     const unsigned char* vb = vc + (bh * a.NB + blk) * (long)(BLK * D);
     const float kscale = ksc[bh * a.NB + blk] * a.scale;
@@ -340,115 +422,128 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
 #pragma unroll
     for (int i = 0; i < DT16; ++i)
       vr[i] = *reinterpret_cast<const u32x4*>(vb + (16 * i + c16) * BLK + 16 * g);
+    const int tok0 = blk * BLK + 16 * g;               // this lane group's 16 tokens
+    const int tok = tok0 + part16 * GP;                // this lane's GP of them
+    float add[GP], pad[GP];
+#pragma unroll
+    for (int i = 0; i < GP; ++i) {
+      const int at = min(tok + i, len - 1);
+      add[i] = bias ? bias[at] : 0.f;
+      pad[i] = kpad ? kpad[at] : 0.f;
+    }
 
-    f32x4 sc[4];
+    f32x16 sc;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 s4 = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < KSTEP; ++s) sc[t] = KFrag<T>::mfma(KFrag<T>::load(kr[t][s]), qf[s], sc[t]);
+      for (int s = 0; s < KSTEP; ++s) s4 = KFrag<T>::mfma(KFrag<T>::load(kr[t][s]), qf[s], s4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[4 * t + r] = s4[r];
     }
-    const int tok0 = blk * BLK + 16 * g;     // this lane group's 16 tokens
+    // this lane's GP scores to the front
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int n = 8; n >= GP; n >>= 1) {
+      const bool upper = part16 & (n / GP);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sc[t][r] *= kscale;
-    if (BIAS) {
-      f32x4 m4[4];
-      mask16(a.bias + b * a.bias_b + hq * a.bias_h, tok0, len, a.mask16, m4);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[t][r] += m4[t][r];
+      for (int i = 0; i < n; ++i) sc[i] = upper ? sc[i + n] : sc[i];
     }
-    unsigned gone = 0;                       // tokens of this lane group that are not there
-    if (KPAD) {
-      f32x4 m4[4];
-      mask16(a.kpad + b * a.kpad_b, tok0, len, a.mask16, m4);
+    bool hole = (blk + 1) * BLK > len;                 // the sequence ends in this block
+    float mx = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sc[t][r] += m4[t][r];
-          gone |= m4[t][r] == -INFINITY ? 1u << (4 * t + r) : 0u;
-        }
+    for (int i = 0; i < GP; ++i) {
+      sc[i] = fmaf(sc[i], kscale, add[i]) + pad[i];
+      const bool gone = tok + i >= len || pad[i] == -INFINITY;
+      sc[i] = gone ? -INFINITY : sc[i];
+      hole |= gone;
+      mx = fmaxf(mx, sc[i]);
     }
-    if ((blk + 1) * BLK > len) {             // the sequence ends in this block
-      const int n = min(max(len - tok0, 0), 16);
-      gone |= 0xffffu & ~((1u << n) - 1u);
-    }
-    if (__any(gone != 0)) {
+    if (__any(hole)) {
       // what is not there counts for nothing whatever its bytes hold, NaN codes
-      // and NaN masks among them
+      // among them
+      unsigned gone = 0xffffu & ~((1u << min(max(len - tok0, 0), 16)) - 1u);
+      if (kpad) {
+#pragma unroll 4
+        for (int j = 0; j < 16; ++j)
+          gone |= kpad[min(tok0 + j, len - 1)] == -INFINITY ? 1u << j : 0u;
+      }
       u32x4 keep;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        unsigned bytes = 0;
+        keep[t] = 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool is_gone = gone >> (4 * t + r) & 1u;
-          if (is_gone) sc[t][r] = -INFINITY;
-          bytes |= is_gone ? 0u : 0xffu << (8 * r);
-        }
-        keep[t] = bytes;
+        for (int r = 0; r < 4; ++r) keep[t] |= gone >> (4 * t + r) & 1u ? 0u : 0xffu << (8 * r);
       }
 #pragma unroll
       for (int i = 0; i < DT16; ++i) vr[i] &= keep;
     }
-    float mx = -INFINITY;
+    if (__any(mx > m + 8.f)) {
+      mx = over_columns<GP>(mx, [](float x, float y) { return fmaxf(x, y); });
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.f : mn)) * LOG2E);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+      for (int i = 0; i < DT16; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[t][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float mn = fmaxf(m, mx);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f((m - ref) * LOG2E);
-    m = mn;
-    l *= alpha;
+        for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    unsigned hi[GP > 1 ? GP / 2 : 1], lo[GP > 1 ? GP / 2 : 1];   // two tokens each
+    if (GP == 1) {
+      const float p = __builtin_amdgcn_exp2f((sc[0] - ref) * LOG2E);
+      l += p;
+      const __bf16 h1 = (__bf16)p;
+      const __bf16 l1 = (__bf16)(p - (float)h1);
+      const int odd = 16 * (c16 & 1);
+      hi[0] = (unsigned)__builtin_bit_cast(unsigned short, h1) << odd;
+      lo[0] = (unsigned)__builtin_bit_cast(unsigned short, l1) << odd;
+    } else {
 #pragma unroll
-    for (int i = 0; i < DT16; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
-    bf16x8 ph[2], pl[2];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f((sc[t][r] - ref) * LOG2E);
-        l += p;
-        const __bf16 hi = (__bf16)p;
-        const __bf16 low = (__bf16)(p - (float)hi);
-        const int e = 4 * (t & 1) + r;
-        ph[t >> 1][e] = !WIDE && lo_half ? low : hi;
-        if (WIDE) pl[t >> 1][e] = low;
-      }
-#pragma unroll
-    for (int i = 0; i < DT16; ++i) {
-      const bf16x8 v0 = v_frag(vr[i][0], vr[i][1], vscale);
-      const bf16x8 v1 = v_frag(vr[i][2], vr[i][3], vscale);
-      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph[0], acc[i], 0, 0, 0);
-      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph[1], acc[i], 0, 0, 0);
-      if (WIDE) {
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl[0], acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl[1], acc[i], 0, 0, 0);
+      for (int i = 0; i < GP / 2; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f((sc[2 * i] - ref) * LOG2E);
+        const float p1 = __builtin_amdgcn_exp2f((sc[2 * i + 1] - ref) * LOG2E);
+        l += p0;
+        l += p1;
+        const bf16x2 h2 = bf16x2{(__bf16)p0, (__bf16)p1};
+        const bf16x2 l2 = bf16x2{(__bf16)(p0 - (float)h2[0]), (__bf16)(p1 - (float)h2[1])};
+        hi[i] = __builtin_bit_cast(unsigned, h2);
+        lo[i] = __builtin_bit_cast(unsigned, l2);
       }
     }
-  }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (!WIDE) {                       // hi and lo columns
+    // tokens 2e, 2e + 1 are this lane's, or 0
+    u32x4 ph[2], pl[2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      constexpr int PAIRS = GP > 1 ? GP / 2 : 1;
+      const bool own = GP > 1 ? part16 == e / PAIRS : part16 >> 1 == e;
+      ph[e >> 2][e & 3] = own ? hi[e % PAIRS] : 0u;
+      pl[e >> 2][e & 3] = own ? lo[e % PAIRS] : 0u;
+    }
 #pragma unroll
     for (int i = 0; i < DT16; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][r] += __shfl_xor(acc[i][r], 8);
+      for (int e = 0; e < 2; ++e) {
+        const bf16x8 v = v_frag(vr[i][2 * e], vr[i][2 * e + 1], vscale);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, ph[e]), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pl[e]), acc[i], 0, 0, 0);
+      }
   }
+  const auto sum = [](float x, float y) { return x + y; };
+  l = over_columns<GP>(l, sum);
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int i = 0; i < DT16; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[i][r] = over_columns<GP>(acc[i][r], sum);
 
   // join the waves
-  __shared__ float so[WAVES][COLS][D + 4];
-  __shared__ float sm[WAVES][COLS], sl[WAVES][COLS];
-  if (c16 < COLS) {
+  __shared__ float so[WAVES][GP][D + 4];
+  __shared__ float sm[WAVES][GP], sl[WAVES][GP];
+  if (c16 < GP) {
     // D layout: column = query, row d = 16i + 4g + r
 #pragma unroll
     for (int i = 0; i < DT16; ++i)
@@ -457,47 +552,62 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
     if (g == 0) { sm[wave][c16] = m; sl[wave][c16] = l; }
   }
   __syncthreads();
-  const int ncol = min(COLS, a.G - q0);
-  for (int e = threadIdx.x; e < ncol * D; e += 256) {
-    const int c = e / D, d = e % D;
+  const int ncol = min(GP, a.G - q0);
+  for (int e = threadIdx.x; e < WAVES / a.share * ncol * D; e += 256) {
+    const int d = e % D, c = e / D % ncol, w0 = e / D / ncol * a.share;
+    const long row = (long)blockIdx.x * (WAVES / a.share) + w0 / a.share;
+    if (row >= a.BH) break;
     float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) mm = fmaxf(mm, sm[w][c]);
+    for (int w = w0; w < w0 + a.share; ++w) mm = fmaxf(mm, sm[w][c]);
     const float ref = mm == -INFINITY ? 0.f : mm;
     float o = 0.f, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = w0; w < w0 + a.share; ++w) {
       const float f = __builtin_amdgcn_exp2f((sm[w][c] - ref) * LOG2E);
       o += so[w][c][d] * f;
       ll += sl[w][c] * f;
     }
-    const int head = h * a.G + q0 + c;
+    const long head = row * a.G + q0 + c;            // of B * Hq
     if (a.nsplit == 1) {
       // l is NaN where a score was: then so is the output
-      out[((long)b * a.Hq + head) * D + d] = DT<T>::from_f32(ll == 0.f ? 0.f : o / ll);
+      out[head * D + d] = DT<T>::from_f32(ll == 0.f ? 0.f : o / ll);
     } else {
-      float* p = part + (((long)b * a.Hq + head) * a.nsplit + split) * (D + 2);
-      p[d] = o;
-      if (d == 0) { p[D] = mm; p[D + 1] = ll; }
+      part[(head * a.nsplit + split) * D + d] = o;
+      if (d == 0) {
+        float* ml = part + (long)a.BH * a.G * a.nsplit * D + (head * a.nsplit + split) * 2;
+        ml[0] = mm;
+        ml[1] = ll;
+      }
     }
   }
 }
 
+// Joins the nsplit parts of each query head: a workgroup of whole waves a head,
+// a thread a d.
 template <typename T, int D>
-__global__ void __launch_bounds__(D) kv8_join_kernel(const float* __restrict__ part,
-                                                     T* __restrict__ out, int nsplit) {
-  const float* p = part + (long)blockIdx.x * nsplit * (D + 2);
-  const int d = threadIdx.x;
-  float mm = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) mm = fmaxf(mm, p[s * (D + 2) + D]);
+__global__ void __launch_bounds__(D < 64 ? 64 : D) kv8_join_kernel(const float* __restrict__ part,
+                                                     T* __restrict__ out, long heads, int nsplit) {
+  __shared__ float f[MAX_SPLIT];
+  const long head = blockIdx.x;
+  const int d = threadIdx.x, lane = d & 63;
+  const float* p = part + head * nsplit * D + min(d, D - 1);
+  const float2* ml = reinterpret_cast<const float2*>(part + heads * nsplit * D) + head * nsplit;
+  float mm = -INFINITY, ll = 0.f;
+  // each wave for itself: a lane a part
+  for (int s = lane; s < nsplit; s += 64) mm = fmaxf(mm, ml[s].x);
+  mm = wave_reduce_max(mm);
   const float ref = mm == -INFINITY ? 0.f : mm;
-  float o = 0.f, ll = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float f = __builtin_amdgcn_exp2f((p[s * (D + 2) + D] - ref) * LOG2E);
-    o += p[s * (D + 2) + d] * f;
-    ll += p[s * (D + 2) + D + 1] * f;
+  for (int s = lane; s < nsplit; s += 64) {
+    const float2 v = ml[s];
+    const float w = __builtin_amdgcn_exp2f((v.x - ref) * LOG2E);
+    f[s] = w;                                        // the same from every wave
+    ll += v.y * w;
   }
-  out[(long)blockIdx.x * D + d] = DT<T>::from_f32(ll == 0.f ? 0.f : o / ll);
+  ll = wave_reduce_sum(ll);
+  __syncthreads();
+  float o = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < nsplit; ++s) o += p[(long)s * D] * f[s];
+  if (d < D) out[head * D + d] = DT<T>::from_f32(ll == 0.f ? 0.f : o / ll);
 }
 
 struct Cache {
@@ -570,6 +680,13 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
   auto stream = at::hip::getCurrentHIPStream().stream();
   const Str3 kst{k.stride(0), k.stride(1), k.stride(2)}, vst{v.stride(0), v.stride(1), v.stride(2)};
 #define APPEND(T, DD)                                                                            \
+  if (S == 1)                                                                                    \
+    hipLaunchKernelGGL((kv8_append_one_kernel<T, DD>), dim3((c.B * c.H + 3) / 4, 2), dim3(256),   \
+                       0, stream, (const T*)k.data_ptr(), (const T*)v.data_ptr(), kst, vst,       \
+                       (unsigned char*)kc.data_ptr(), (unsigned char*)vc.data_ptr(),              \
+                       ks.data_ptr<float>(), vs.data_ptr<float>(), st, ct, (int)(c.B * c.H),      \
+                       (int)c.H, (int)c.NB);                                                      \
+  else                                                                                            \
   hipLaunchKernelGGL((kv8_append_kernel<T, DD>), dim3(c.B* c.H* NW, 2), dim3(256), 0, stream,     \
                      (const T*)k.data_ptr(), (const T*)v.data_ptr(), kst, vst,                    \
                      (unsigned char*)kc.data_ptr(), (unsigned char*)vc.data_ptr(),                \
@@ -577,9 +694,9 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
                      (int)c.NB, (int)NW)
 #define BY_DIM(T, F)                            \
   do {                                          \
-    if (c.D == 32) F(T, 32);                    \
-    else if (c.D == 64) F(T, 64);               \
-    else F(T, 128);                             \
+    if (c.D == 32) { F(T, 32); }                \
+    else if (c.D == 64) { F(T, 64); }           \
+    else { F(T, 128); }                         \
   } while (0)
   if (k.scalar_type() == torch::kBFloat16) BY_DIM(__hip_bfloat16, APPEND);
   else if (k.scalar_type() == torch::kHalf) BY_DIM(__half, APPEND);
@@ -629,22 +746,19 @@ torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torc
   if (c.B == 0 || Hq == 0) return out;
   if (max_len == 0) return out.zero_();
   const int G = Hq / c.H;
-  const bool wide = G > 8;
-  const int nz = (G + (wide ? 15 : 7)) / (wide ? 16 : 8);
+  const int GP = G > 8 ? 16 : G > 4 ? 8 : G > 2 ? 4 : G;
+  const int nz = (G + GP - 1) / GP;
   const long nblk = (max_len + BLK - 1) / BLK;
-  // Enough workgroups to fill 256 CUs a few times over, and at least two
-  // blocks of tokens for each of a workgroup's four waves.
-  long nsplit = std::max(1L, std::min(1024 / std::max(1L, c.B * c.H * nz), nblk / 8));
+  long nsplit = nblk < 32 ? 1 : std::max(1L, std::min({512 / (c.B * c.H * nz), nblk / 8, (long)MAX_SPLIT}));
+  if (const char* ev = getenv("KV8_SPLIT")) nsplit = std::max(1L, std::min({atol(ev) / std::max(1L, c.B * c.H * nz), nblk / 4, (long)MAX_SPLIT}));
   TORCH_CHECK(c.B * c.H < (1L << 31) && nz < 65536, "kv8_attn: too many heads");
   a.scale = (float)scale;
-  a.Hq = Hq; a.H = c.H; a.G = G; a.NB = c.NB; a.max_len = max_len; a.nsplit = nsplit;
+  a.share = nsplit > 1 || nblk > 3 ? 4 : nblk > 1 ? 2 : 1;
+  a.BH = c.B * c.H; a.Hq = Hq; a.H = c.H; a.G = G; a.NB = c.NB; a.max_len = max_len; a.nsplit = nsplit;
   torch::Tensor part;
   if (nsplit > 1) part = torch::empty({c.B * Hq * nsplit * (c.D + 2)}, ks.options());
   auto stream = at::hip::getCurrentHIPStream().stream();
-  const dim3 grid(c.B * c.H, nsplit, nz);
-  a.mask16 = (!a.bias || (reinterpret_cast<uintptr_t>(a.bias) % 16 == 0 && a.bias_b % 4 == 0 &&
-                          a.bias_h % 4 == 0)) &&
-             (!a.kpad || (reinterpret_cast<uintptr_t>(a.kpad) % 16 == 0 && a.kpad_b % 4 == 0));
+  const dim3 grid((c.B * c.H + 4 / a.share - 1) / (4 / a.share), nsplit, nz);
   auto run = [&](auto kernel, auto* type) {
     using T = std::remove_pointer_t<decltype(type)>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const T*)q.data_ptr(),
@@ -656,21 +770,15 @@ torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torc
 #define ATTN(T, DD)                                                                              \
   do {                                                                                           \
     T* type = nullptr;                                                                           \
-    if (a.bias && a.kpad)                                                                        \
-      wide ? run(kv8_attn_kernel<T, DD, true, true, true>, type)                                 \
-           : run(kv8_attn_kernel<T, DD, false, true, true>, type);                               \
-    else if (a.bias)                                                                             \
-      wide ? run(kv8_attn_kernel<T, DD, true, true, false>, type)                                \
-           : run(kv8_attn_kernel<T, DD, false, true, false>, type);                              \
-    else if (a.kpad)                                                                             \
-      wide ? run(kv8_attn_kernel<T, DD, true, false, true>, type)                                \
-           : run(kv8_attn_kernel<T, DD, false, false, true>, type);                              \
-    else                                                                                         \
-      wide ? run(kv8_attn_kernel<T, DD, true, false, false>, type)                               \
-           : run(kv8_attn_kernel<T, DD, false, false, false>, type);                             \
+    if (GP == 1) run(kv8_attn_kernel<T, DD, 1>, type);                                           \
+    else if (GP == 2) run(kv8_attn_kernel<T, DD, 2>, type);                                      \
+    else if (GP == 4) run(kv8_attn_kernel<T, DD, 4>, type);                                      \
+    else if (GP == 8) run(kv8_attn_kernel<T, DD, 8>, type);                                      \
+    else run(kv8_attn_kernel<T, DD, 16>, type);                                                  \
     if (nsplit > 1)                                                                              \
-      hipLaunchKernelGGL((kv8_join_kernel<T, DD>), dim3(c.B* Hq), dim3(DD), 0, stream,           \
-                         part.data_ptr<float>(), (T*)out.data_ptr(), (int)nsplit);               \
+      hipLaunchKernelGGL((kv8_join_kernel<T, DD>), dim3(c.B* Hq), dim3(DD < 64 ? 64 : DD), 0,    \
+                         stream, part.data_ptr<float>(), (T*)out.data_ptr(), c.B* Hq,            \
+                         (int)nsplit);                                                           \
   } while (0)
   if (q.scalar_type() == torch::kBFloat16) BY_DIM(__hip_bfloat16, ATTN);
   else if (q.scalar_type() == torch::kHalf) BY_DIM(__half, ATTN);

@@ -68,71 +68,324 @@ DEVINL float group_scale(int e, int row_e) {
   return __builtin_bit_cast(float, (unsigned)(d + 127) << 23);
 }
 
+// 2^(e - 127); byte 0 is the subnormal 2^-127, 255 is no scale
+DEVINL float row_scale(int e) {
+  return __builtin_bit_cast(float, e ? (unsigned)e << 23 : 0x00400000u);
+}
+
+struct Args {
+  const unsigned char *codes, *exps, *row_exp;
+  int M, N, K;
+  long ldx;
+};
+
 // ---------------------------------------------------------------------------
-// Up to 16*MT rows, x straight from the caches: one wave owns 16 outputs and
-// every WAVES-th 128-wide piece of K, the block's waves are summed through LDS
-// in wave order (the same sum every time).
+// Up to 16*MT rows, x straight from the caches: one wave owns 16*NT outputs
+// and every WAVES-th 128-wide piece of K, the next piece's weights and x on
+// their way while this one is multiplied.  The block's waves are summed through
+// LDS in wave order (the same sum every time).
 // ---------------------------------------------------------------------------
-template <typename T, int MT, int WAVES>
+template <typename T, int MT, int NT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
-w4_few_rows(const T* __restrict__ x, const unsigned char* __restrict__ codes,
-            const unsigned char* __restrict__ exps, const unsigned char* __restrict__ row_exp,
-            T* __restrict__ y, int M, int N, int K, long ldx) {
+w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
+  using vec = typename Frag<T>::vec;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
-  const int n = blockIdx.x * 16 + c16;
-  const int m0 = blockIdx.y * (16 * MT);
-  const bool n_ok = n < N;
-  const int row_e = n_ok ? row_exp[n] : 127;
-  const unsigned char* crow = codes + (long)(n_ok ? n : 0) * (K >> 1);
-  const unsigned char* erow = exps + (long)(n_ok ? n : 0) * (K >> 5);
-
-  f32x4 acc[MT];
+  const int n0 = blockIdx.x * (16 * NT) + c16, m0 = blockIdx.y * (16 * MT) + c16;
+  int row_e[NT];
+  const unsigned char *crow[NT], *erow[NT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) {
+    const int n = min(n0 + 16 * t, a.N - 1);      // the last row again: not stored
+    row_e[t] = a.row_exp[n];
+    crow[t] = a.codes + (long)n * (a.K >> 1);
+    erow[t] = a.exps + (long)n * (a.K >> 5);
+  }
 
-  for (int k0 = wave * 128; k0 < K; k0 += WAVES * 128) {
-    const int k = k0 + 32 * g;
-    const bool k_ok = k < K;              // K is a multiple of 32
-    u32x4 w = u32x4{0u, 0u, 0u, 0u};
-    float scale = 1.f;
-    if (k_ok && n_ok) {
-      w = *reinterpret_cast<const u32x4*>(crow + (k >> 1));
-      scale = group_scale(erow[k >> 5], row_e);
+  struct Piece {
+    u32x4 w[NT], x[MT][4];
+    int e[NT];
+  };
+  auto load = [&](int k0) {
+    Piece p;
+    const int k = k0 + 32 * g;                    // K is a multiple of 32
+    const bool k_ok = k < a.K;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      p.w[t] = u32x4{0u, 0u, 0u, 0u};
+      p.e[t] = 127;
+      if (k_ok) {
+        p.w[t] = *reinterpret_cast<const u32x4*>(crow[t] + (k >> 1));
+        p.e[t] = erow[t][k >> 5];
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const typename Frag<T>::vec wf = decode8<T>(w[i], scale);
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int m = m0 + 16 * t + c16;
-        u32x4 xv = u32x4{0u, 0u, 0u, 0u};
-        if (k_ok && m < M) xv = *reinterpret_cast<const u32x4*>(x + m * ldx + k + 8 * i);
-        acc[t] = Frag<T>::mfma(__builtin_bit_cast(typename Frag<T>::vec, xv), wf, acc[t]);
+      for (int i = 0; i < 4; ++i) {
+        p.x[t][i] = u32x4{0u, 0u, 0u, 0u};
+        if (k_ok && m0 + 16 * t < a.M)
+          p.x[t][i] = *reinterpret_cast<const u32x4*>(x + (m0 + 16 * t) * a.ldx + k + 8 * i);
+      }
+    return p;
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  Piece next = load(wave * 128);
+  for (int k0 = wave * 128; k0 < a.K; k0 += WAVES * 128) {
+    const Piece p = next;
+    if (k0 + WAVES * 128 < a.K) next = load(k0 + WAVES * 128);
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const float scale = group_scale(p.e[u], row_e[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const vec wf = decode8<T>(p.w[u][i], scale);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          acc[t][u] = Frag<T>::mfma(__builtin_bit_cast(vec, p.x[t][i]), wf, acc[t][u]);
       }
     }
   }
 
-  __shared__ f32x4 part[WAVES][MT][64];
+  __shared__ f32x4 part[WAVES][MT * NT][64];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) part[wave][t * NT + u][lane] = acc[t][u];
   __syncthreads();
   // D layout: column n = lane%16, row m = 4*(lane/16) + r
-  // 2^(row_e - 127); byte 0 is the subnormal 2^-127
-  const float back = __builtin_bit_cast(float, row_e ? (unsigned)row_e << 23 : 0x00400000u);
-  for (int t = wave; t < MT; t += WAVES) {
-    f32x4 s = part[0][t][lane];
+  for (int q = wave; q < MT * NT; q += WAVES) {
+    const int t = q / NT, n = n0 + 16 * (q % NT);
+    f32x4 s = part[0][q][lane];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) {
-      const f32x4 p = part[v][t][lane];
+      const f32x4 p = part[v][q][lane];
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] += p[r];
     }
+    if (n >= a.N) continue;
+    const float back = row_scale(a.row_exp[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int m = m0 + 16 * t + 4 * g + r;
-      if (n_ok && m < M) y[(long)m * N + n] = DT<T>::from_f32(s[r] * back);
+      const int m = m0 - c16 + 16 * t + 4 * g + r;
+      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
     }
+  }
+}
+
+// Up to 16 rows of x in LDS.
+template <typename T, int NT, int U, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64)
+w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
+  using vec = typename Frag<T>::vec;
+  extern __shared__ char shared[];
+  T* xs = reinterpret_cast<T*>(shared);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, c16 = lane & 15;
+  const int n0 = blockIdx.x * (16 * NT) + c16;
+  const int LD = a.K + 8;
+  int row_e[NT];
+  const unsigned char *crow[NT], *erow[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = min(n0 + 16 * t, a.N - 1);      // the last row again: not stored
+    row_e[t] = a.row_exp[n];
+    crow[t] = a.codes + (long)n * (a.K >> 1);
+    erow[t] = a.exps + (long)n * (a.K >> 5);
+  }
+  struct Piece {
+    u32x4 w[U][NT];
+    int e[U][NT];
+  };
+  auto load = [&](int k0) {
+    Piece p;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = k0 + 128 * j + 32 * g;          // K is a multiple of 32
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        p.w[j][t] = u32x4{0u, 0u, 0u, 0u};
+        p.e[j][t] = 127;
+        if (k < a.K) {
+          p.w[j][t] = *reinterpret_cast<const u32x4*>(crow[t] + (k >> 1));
+          p.e[j][t] = erow[t][k >> 5];
+        }
+      }
+    }
+    return p;
+  };
+  constexpr int RUN = WAVES * 128 * U;
+  Piece next = load(wave * 128 * U);
+  for (int i = threadIdx.x * 8; i < a.M * a.K; i += WAVES * 64 * 8) {
+    const int m = i / a.K, k = i - m * a.K;
+    *reinterpret_cast<u32x4*>(xs + m * LD + k) = *reinterpret_cast<const u32x4*>(x + m * a.ldx + k);
+  }
+  __syncthreads();
+  f32x4 acc[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T* xrow = xs + min(c16, a.M - 1) * LD;
+  for (int k0 = wave * 128 * U; k0 < a.K; k0 += RUN) {
+    const Piece p = next;
+    if (k0 + RUN < a.K) next = load(k0 + RUN);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = min(k0 + 128 * j + 32 * g, a.K - 32);
+      float scale[NT];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) scale[u] = group_scale(p.e[j][u], row_e[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const vec xf = *reinterpret_cast<const vec*>(xrow + k + 8 * i);
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+          acc[u] = Frag<T>::mfma(xf, decode8<T>(p.w[j][u][i], scale[u]), acc[u]);
+      }
+    }
+  }
+  __shared__ f32x4 part[WAVES][NT][64];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) part[wave][u][lane] = acc[u];
+  __syncthreads();
+  for (int q = wave; q < NT; q += WAVES) {
+    const int n = n0 + 16 * q;
+    f32x4 s = part[0][q][lane];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) {
+      const f32x4 p = part[v][q][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += p[r];
+    }
+    if (n >= a.N) continue;
+    const float back = row_scale(a.row_exp[n]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = 4 * g + r;
+      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of 2 x 2 waves makes 2*16*MT rows by 2*16*NT outputs.
+// x goes through LDS, 128 of K at a time in two buffers (two pieces are on
+// their way in registers while one is multiplied, rows 16 bytes apart from a
+// multiple of 256 so that 16 rows at one k lie in different banks); weights
+// go from memory to registers as above, converted once for MT tiles of rows.
+// ---------------------------------------------------------------------------
+template <typename T, int MT, int NT, int WN>
+__global__ void __launch_bounds__(128 * WN)
+w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
+  using vec = typename Frag<T>::vec;
+  constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * NT * WN, KC = 128, LD = KC + 8;
+  constexpr int LOADS = BM * KC / 8 / THREADS;       // 16-byte pieces of x a thread brings
+  __shared__ alignas(16) T lds[2][BM * LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, c16 = lane & 15;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int m_at = blockIdx.x * BM, n0 = blockIdx.y * BN + wn * 16 * NT + c16;
+  int row_e[NT];
+  const unsigned char *crow[NT], *erow[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = min(n0 + 16 * t, a.N - 1);      // the last row again: not stored
+    row_e[t] = a.row_exp[n];
+    crow[t] = a.codes + (long)n * (a.K >> 1);
+    erow[t] = a.exps + (long)n * (a.K >> 5);
+  }
+  struct Piece {
+    u32x4 x[LOADS], w[NT];
+    int e[NT];
+  } ahead[2];
+  auto load = [&](Piece& p, int k0) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int piece = threadIdx.x + THREADS * i;
+      const int m = m_at + piece / (KC / 8), k = k0 + piece % (KC / 8) * 8;
+      p.x[i] = u32x4{0u, 0u, 0u, 0u};
+      if (m < a.M && k < a.K) p.x[i] = *reinterpret_cast<const u32x4*>(x + m * a.ldx + k);
+    }
+    const int k = k0 + 32 * g;                    // K is a multiple of 32
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      p.w[t] = u32x4{0u, 0u, 0u, 0u};
+      p.e[t] = 127;
+      if (k < a.K) {
+        p.w[t] = *reinterpret_cast<const u32x4*>(crow[t] + (k >> 1));
+        p.e[t] = erow[t][k >> 5];
+      }
+    }
+  };
+  auto stage = [&](const Piece& p, int buf) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int piece = threadIdx.x + THREADS * i;
+      *reinterpret_cast<u32x4*>(&lds[buf][piece / (KC / 8) * LD + piece % (KC / 8) * 8]) = p.x[i];
+    }
+  };
+  // orders LDS alone: a plain barrier would wait for the loads on their way
+  auto lds_barrier = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // multiplies the piece in `buf`, whose weights are in `now`, while that after
+  // the next is loaded
+  auto step = [&](int k0, Piece& now, const Piece& next, int buf) {
+    u32x4 w[NT];
+    float scale[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) { w[u] = now.w[u]; scale[u] = group_scale(now.e[u], row_e[u]); }
+    if (k0 + 2 * KC < a.K) load(now, k0 + 2 * KC);
+    const T* row = &lds[buf][(wm * 16 * MT + c16) * LD + 32 * g];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      vec xf[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xf[t] = *reinterpret_cast<const vec*>(row + 16 * t * LD + 8 * i);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const vec wf = decode8<T>(w[u][i], scale[u]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t][u] = Frag<T>::mfma(xf[t], wf, acc[t][u]);
+      }
+    }
+    if (k0 + KC < a.K) stage(next, buf ^ 1);
+    lds_barrier();
+  };
+  load(ahead[0], 0);
+  if (KC < a.K) load(ahead[1], KC);
+  stage(ahead[0], 0);
+  lds_barrier();
+  for (int k0 = 0; k0 < a.K; k0 += 2 * KC) {
+    step(k0, ahead[0], ahead[1], 0);
+    if (k0 + KC < a.K) step(k0 + KC, ahead[1], ahead[0], 1);
+  }
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const int n = n0 + 16 * u;
+    if (n >= a.N) continue;
+    const float back = row_scale(row_e[u]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m_at + wm * 16 * MT + 16 * t + 4 * g + r;
+        if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(acc[t][u][r] * back);
+      }
   }
 }
 
@@ -147,8 +400,8 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
                   exps.size(1) * 32 == K && row_exp.size(0) == N,
               "w4_linear: x has ", K, " inputs, codes ", codes.size(1) * 2, ", exps ",
               exps.size(1) * 32);
-  // 65535 blocks of 64 rows
-  TORCH_CHECK(M < (1L << 22) - 64 && N < (1L << 31) && K < (1L << 30), "w4_linear: too large");
+  // a grid's second dimension is 16 bits wide: blocks of 16 rows, of 32 outputs
+  TORCH_CHECK(M < (1L << 31) - 256 && N < 65535L * 32 && K < (1L << 30), "w4_linear: too large");
   for (const auto& t : {codes, exps, row_exp})
     TORCH_CHECK(t.scalar_type() == torch::kByte && t.is_contiguous() && t.device() == x.device(),
                 "w4_linear: codes and exponents must be contiguous uint8 on x's device");
@@ -162,17 +415,65 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
       reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0)
     x = x.clone(at::MemoryFormat::Contiguous);
   auto stream = at::hip::getCurrentHIPStream().stream();
+  const Args a{codes.data_ptr<unsigned char>(), exps.data_ptr<unsigned char>(),
+               row_exp.data_ptr<unsigned char>(), (int)M, (int)N, (int)K, (long)x.stride(0)};
+  const char* ev = getenv("W4_CFG");
+  const int cfg = ev ? atoi(ev) : 0;
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    const dim3 grid((N + 15) / 16, M <= 16 ? 1 : (M + 63) / 64);
-    auto call = [&](auto kernel, int waves) {
-      hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), 0, stream, (const T*)x.data_ptr(),
-                         codes.data_ptr<unsigned char>(), exps.data_ptr<unsigned char>(),
-                         row_exp.data_ptr<unsigned char>(), (T*)y.data_ptr(), (int)M, (int)N,
-                         (int)K, (long)x.stride(0));
+    auto few = [&](auto kernel, int mt, int nt, int waves) {
+      hipLaunchKernelGGL(kernel, dim3((N + 16 * nt - 1) / (16 * nt), (M + 16 * mt - 1) / (16 * mt)),
+                         dim3(waves * 64), 0, stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
     };
-    if (M <= 16) call(w4_few_rows<T, 1, 8>, 8);
-    else call(w4_few_rows<T, 4, 4>, 4);
+    auto many = [&](auto kernel, int mt, int nt, int wn) {
+      hipLaunchKernelGGL(kernel, dim3((M + 32 * mt - 1) / (32 * mt), (N + 16 * nt * wn - 1) / (16 * nt * wn)),
+                         dim3(128 * wn), 0, stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
+    };
+    auto lds = [&](auto kernel, int nt, int waves) {
+      hipLaunchKernelGGL(kernel, dim3((N + 16 * nt - 1) / (16 * nt)), dim3(waves * 64), M * (K + 8) * 2,
+                         stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
+    };
+    switch (cfg) {
+      case 21: lds(w4_lds_rows<T, 1, 1, 8>, 1, 8); return;
+      case 22: lds(w4_lds_rows<T, 1, 2, 8>, 1, 8); return;
+      case 23: lds(w4_lds_rows<T, 1, 4, 8>, 1, 8); return;
+      case 24: lds(w4_lds_rows<T, 1, 1, 16>, 1, 16); return;
+      case 25: lds(w4_lds_rows<T, 1, 2, 16>, 1, 16); return;
+      case 26: lds(w4_lds_rows<T, 2, 1, 8>, 2, 8); return;
+      case 27: lds(w4_lds_rows<T, 2, 2, 8>, 2, 8); return;
+      case 28: lds(w4_lds_rows<T, 1, 2, 4>, 1, 4); return;
+      case 29: lds(w4_lds_rows<T, 1, 4, 4>, 1, 4); return;
+      case 30: lds(w4_lds_rows<T, 2, 2, 4>, 2, 4); return;
+      case 31: lds(w4_lds_rows<T, 2, 4, 4>, 2, 4); return;
+      case 32: lds(w4_lds_rows<T, 2, 2, 16>, 2, 16); return;
+      case 1: few(w4_few_rows<T, 1, 1, 8>, 1, 1, 8); return;
+      case 2: few(w4_few_rows<T, 1, 2, 8>, 1, 2, 8); return;
+      case 3: few(w4_few_rows<T, 1, 4, 8>, 1, 4, 8); return;
+      case 4: few(w4_few_rows<T, 1, 2, 4>, 1, 2, 4); return;
+      case 5: few(w4_few_rows<T, 1, 4, 4>, 1, 4, 4); return;
+      case 6: few(w4_few_rows<T, 2, 2, 4>, 2, 2, 4); return;
+      case 7: few(w4_few_rows<T, 2, 1, 8>, 2, 1, 8); return;
+      case 8: few(w4_few_rows<T, 4, 1, 4>, 4, 1, 4); return;
+      case 9: few(w4_few_rows<T, 2, 4, 4>, 2, 4, 4); return;
+      case 10: few(w4_few_rows<T, 1, 1, 4>, 1, 1, 4); return;
+      case 11: many(w4_many_rows<T, 1, 1, 2>, 1, 1, 2); return;
+      case 12: many(w4_many_rows<T, 2, 2, 2>, 2, 2, 2); return;
+      case 13: many(w4_many_rows<T, 4, 2, 2>, 4, 2, 2); return;
+      case 14: many(w4_many_rows<T, 2, 4, 2>, 2, 4, 2); return;
+      case 15: many(w4_many_rows<T, 4, 4, 2>, 4, 4, 2); return;
+      case 16: many(w4_many_rows<T, 1, 2, 2>, 1, 2, 2); return;
+      case 17: many(w4_many_rows<T, 2, 1, 2>, 2, 1, 2); return;
+      case 18: many(w4_many_rows<T, 4, 1, 2>, 4, 1, 2); return;
+      case 41: many(w4_many_rows<T, 4, 2, 4>, 4, 2, 4); return;
+      case 42: many(w4_many_rows<T, 4, 1, 4>, 4, 1, 4); return;
+      case 43: many(w4_many_rows<T, 2, 2, 4>, 2, 2, 4); return;
+      case 44: many(w4_many_rows<T, 2, 1, 4>, 2, 1, 4); return;
+      case 45: many(w4_many_rows<T, 4, 4, 4>, 4, 4, 4); return;
+      case 46: many(w4_many_rows<T, 1, 1, 4>, 1, 1, 4); return;
+      case 47: many(w4_many_rows<T, 1, 2, 4>, 1, 2, 4); return;
+    }
+    if (M <= 16) few(w4_few_rows<T, 1, 1, 8>, 1, 1, 8);
+    else many(w4_many_rows<T, 2, 2, 2>, 2, 2, 2);
   };
   if (x.scalar_type() == torch::kBFloat16) go(__hip_bfloat16());
   else if (x.scalar_type() == torch::kHalf) go(__half());
