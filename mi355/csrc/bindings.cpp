@@ -85,7 +85,7 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
                 c10::optional<torch::Tensor> counts);
 torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks,
                        torch::Tensor vs, c10::optional<torch::Tensor> lengths, long length,
-                       long max_len, c10::optional<torch::Tensor> bias,
+                       long max_len, bool has_max_len, c10::optional<torch::Tensor> bias,
                        c10::optional<torch::Tensor> kpad, double scale);
 torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
                             c10::optional<torch::Tensor> temperatures, double temperature,

@@ -109,3 +109,15 @@ DEVINL float hash_u01(long long seed, long long idx) {
                   hipGetErrorString(e_));                            \
     }                                                                \
   } while (0)
+
+// A refused argument: ValueError in Python (in files that include
+// torch/extension.h).
+#define VALUE_CHECK(cond, ...) \
+  do {                         \
+    if (!(cond)) throw pybind11::value_error(c10::str(__VA_ARGS__)); \
+  } while (0)
+
+// Operators without a backward pass refuse inputs that ask for a gradient.
+#define NO_GRAD_CHECK(t, what)                                     \
+  TORCH_CHECK(!(t).requires_grad() || !at::GradMode::is_enabled(), \
+              what " has no backward pass: call it under torch.no_grad()")

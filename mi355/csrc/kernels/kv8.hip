@@ -611,41 +611,52 @@ __global__ void __launch_bounds__(D < 64 ? 64 : D) kv8_join_kernel(const float* 
 }
 
 struct Cache {
-  torch::Tensor k, v, ks, vs;
+  const torch::Tensor &k, &v, &ks, &vs;
   long B, H, NB, D;
 };
 
 Cache check_cache(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ks,
                   const torch::Tensor& vs) {
-  TORCH_CHECK(k.dim() == 4 && v.dim() == 5 && ks.dim() == 3 && vs.dim() == 3,
+  VALUE_CHECK(k.dim() == 4 && v.dim() == 5 && ks.dim() == 3 && vs.dim() == 3,
               "kv8: k (B,H,NB*64,D), v (B,H,NB,D,64), scales (B,H,NB)");
-  Cache c{k, v, ks, vs, v.size(0), v.size(1), v.size(2), v.size(3)};
-  TORCH_CHECK(v.size(4) == BLK && k.size(0) == c.B && k.size(1) == c.H &&
+  const Cache c{k, v, ks, vs, v.size(0), v.size(1), v.size(2), v.size(3)};
+  VALUE_CHECK(v.size(4) == BLK && k.size(0) == c.B && k.size(1) == c.H &&
                   k.size(2) == c.NB * BLK && k.size(3) == c.D,
               "kv8: k and v are not of one cache");
-  TORCH_CHECK(c.D == 32 || c.D == 64 || c.D == 128, "kv8: head dim 32, 64 or 128, got ", c.D);
-  for (const auto& s : {ks, vs})
-    TORCH_CHECK(s.size(0) == c.B && s.size(1) == c.H && s.size(2) == c.NB && s.is_contiguous() &&
-                    s.scalar_type() == torch::kFloat && s.device() == k.device(),
+  VALUE_CHECK(c.D == 32 || c.D == 64 || c.D == 128, "kv8: head dim 32, 64 or 128, got ", c.D);
+  for (const auto* s : {&ks, &vs})
+    VALUE_CHECK(s->size(0) == c.B && s->size(1) == c.H && s->size(2) == c.NB && s->is_contiguous() &&
+                    s->scalar_type() == torch::kFloat && s->device() == k.device(),
                 "kv8: scales must be contiguous fp32 (B,H,NB) on the cache's device");
-  for (const auto& t : {k, v})
-    TORCH_CHECK(t.is_contiguous() && t.element_size() == 1 && t.is_cuda() &&
-                    t.device() == k.device() &&
-                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+  for (const auto* t : {&k, &v})
+    VALUE_CHECK(t->is_contiguous() && t->element_size() == 1 && t->is_cuda() &&
+                    t->device() == k.device() &&
+                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
                 "kv8: codes must be contiguous 8-bit device tensors, 16-byte aligned");
-  TORCH_CHECK(c.NB < (1L << 24) && c.B * c.H < (1L << 31), "kv8: cache too large");
+  VALUE_CHECK(c.NB < (1L << 24) && c.B * c.H < (1L << 31), "kv8: cache too large");
   return c;
 }
 
-PerSeq per_seq(const c10::optional<torch::Tensor>& each, long all, const Cache& c, const char* what) {
+// `each`, if given, as int32 (kept alive by the caller's tensor)
+PerSeq per_seq(c10::optional<torch::Tensor>& each, long all, const Cache& c, const char* what) {
   if (each.has_value() && each->defined()) {
-    TORCH_CHECK(each->dim() == 1 && each->size(0) == c.B && each->scalar_type() == torch::kInt &&
-                    each->is_contiguous() && each->device() == c.k.device(),
-                "kv8: ", what, " must be an int or a contiguous int32 (B,) tensor on the cache's device");
+    VALUE_CHECK(each->dim() == 1 && each->size(0) == c.B && each->device() == c.k.device() &&
+                    !each->is_floating_point(),
+                "kv8: ", what, " must be a number or an int32 (", c.B, ",) tensor on ",
+                c.k.device(), ", got ", each->sizes(), " on ", each->device());
+    if (each->scalar_type() != torch::kInt || !each->is_contiguous())
+      each = each->to(torch::kInt).contiguous();
     return {each->data_ptr<int>(), 0};
   }
-  TORCH_CHECK(all >= 0 && all < (1L << 30), "kv8: ", what, " out of range: ", all);
+  VALUE_CHECK(all >= 0 && all < (1L << 30), "kv8: ", what, " out of range: ", all);
   return {nullptr, (int)all};
+}
+
+void check_tokens(const torch::Tensor& t, const Cache& c, const char* what) {
+  VALUE_CHECK(t.device() == c.k.device(), what, ": tokens on ", t.device(), ", cache on ", c.k.device());
+  VALUE_CHECK(t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kHalf, what,
+              " takes bf16 or fp16 on a GPU, got ", t.scalar_type());
+  NO_GRAD_CHECK(t, "an 8-bit cache");
 }
 
 // (B,H,S,D) with D contiguous and every row 16-byte aligned
@@ -661,22 +672,23 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
                 torch::Tensor ks, torch::Tensor vs, c10::optional<torch::Tensor> starts, long start,
                 c10::optional<torch::Tensor> counts) {
   const Cache c = check_cache(kc, vc, ks, vs);
-  for (const auto& t : {k, v})
-    TORCH_CHECK(t.dim() == 4 && t.size(0) == c.B && t.size(1) == c.H && t.size(3) == c.D &&
-                    t.size(2) == k.size(2) && t.device() == kc.device() &&
-                    t.scalar_type() == k.scalar_type(),
-                "kv8_append: k and v must be (B,H,S,D) of one type on the cache's device");
+  check_tokens(k, c, "kv8_append");
+  check_tokens(v, c, "kv8_append");
+  VALUE_CHECK(k.dim() == 4 && k.size(0) == c.B && k.size(1) == c.H && k.size(3) == c.D &&
+                  v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
+              "kv8_append: k ", k.sizes(), " and v ", v.sizes(), " of one type do not fit a cache of ",
+              kc.sizes());
   const long S = k.size(2);
+  c10::DeviceGuard guard(kc.device());
   const PerSeq st = per_seq(starts, start, c, "start");
-  TORCH_CHECK(st.each || start + S <= c.NB * BLK, "kv8_append: ", start, " + ", S,
-              " tokens do not fit a cache of ", c.NB * BLK);
+  VALUE_CHECK(st.each || start + S <= c.NB * BLK, "kv8_append: ", S, " tokens at ", start,
+              " do not fit a cache of ", c.NB * BLK);
   const PerSeq ct = per_seq(counts, S, c, "counts");
   if (S == 0 || c.B * c.H == 0) return;
-  c10::DeviceGuard guard(kc.device());
   k = rows16(k);
   v = rows16(v);
   const long NW = (S + BLK - 2) / BLK + 1;
-  TORCH_CHECK(c.B * c.H * NW < (1L << 31), "kv8_append: too many tokens at once");
+  VALUE_CHECK(c.B * c.H * NW < (1L << 31), "kv8_append: too many tokens at once");
   auto stream = at::hip::getCurrentHIPStream().stream();
   const Str3 kst{k.stride(0), k.stride(1), k.stride(2)}, vst{v.stride(0), v.stride(1), v.stride(2)};
 #define APPEND(T, DD)                                                                            \
@@ -699,50 +711,55 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
     else { F(T, 128); }                         \
   } while (0)
   if (k.scalar_type() == torch::kBFloat16) BY_DIM(__hip_bfloat16, APPEND);
-  else if (k.scalar_type() == torch::kHalf) BY_DIM(__half, APPEND);
-  else TORCH_CHECK(false, "kv8_append: bf16 or fp16 tokens, got ", k.scalar_type());
+  else BY_DIM(__half, APPEND);
 #undef APPEND
   HIP_CHECK_KERNEL();
 }
 
 torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks,
                        torch::Tensor vs, c10::optional<torch::Tensor> lengths, long length,
-                       long max_len, c10::optional<torch::Tensor> bias,
+                       long max_len, bool has_max_len, c10::optional<torch::Tensor> bias,
                        c10::optional<torch::Tensor> kpad, double scale) {
   const Cache c = check_cache(kc, vc, ks, vs);
-  TORCH_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(2) == 1 && q.size(3) == c.D &&
-                  q.device() == kc.device(),
-              "kv8_attn: q must be (B,Hq,1,D) on the cache's device");
-  const long Hq = q.size(1);
-  TORCH_CHECK(c.H > 0 && Hq % c.H == 0, "kv8_attn: ", Hq, " query heads over ", c.H, " cache heads");
+  check_tokens(q, c, "decode_attention_kv8");
+  VALUE_CHECK(q.dim() == 4 && q.size(0) == c.B && q.size(2) == 1 && q.size(3) == c.D && c.H > 0 &&
+                  q.size(1) % c.H == 0,
+              "decode_attention_kv8: q ", q.sizes(), " does not fit a cache of ", kc.sizes());
+  const long Hq = q.size(1), cap = c.NB * BLK;
+  c10::DeviceGuard guard(kc.device());
   const PerSeq ln = per_seq(lengths, length, c, "lengths");
-  TORCH_CHECK(ln.each || length <= c.NB * BLK, "kv8_attn: length ", length,
-              " over the cache's capacity ", c.NB * BLK);
-  max_len = std::min(max_len, c.NB * BLK);
-  TORCH_CHECK(max_len >= 0 && (ln.each || max_len >= length), "kv8_attn: max_len ", max_len,
-              " under the length");
+  VALUE_CHECK(ln.each || length <= cap, "decode_attention_kv8: length ", length, " in a cache of ", cap);
+  VALUE_CHECK(!has_max_len || (max_len >= 0 && (ln.each || max_len >= length)),
+              "decode_attention_kv8: max_len ", max_len, " under the length");
+  if (!has_max_len) max_len = ln.each ? cap : length;
+  max_len = std::min(max_len, cap);
   AttnArgs a{};
+  torch::Tensor masks[2];
+  auto mask = [&](c10::optional<torch::Tensor>& t, int i, const char* what) -> const torch::Tensor& {
+    NO_GRAD_CHECK(*t, "decode_attention_kv8");
+    VALUE_CHECK(t->device() == kc.device() && t->size(-1) >= max_len, "decode_attention_kv8: ", what, " ",
+                t->sizes(), " on ", t->device(), " for max_len ", max_len, " on ", kc.device());
+    masks[i] = t->scalar_type() == torch::kFloat && t->stride(-1) == 1 ? *t : t->to(torch::kFloat).contiguous();
+    return masks[i];
+  };
   if (bias.has_value() && bias->defined()) {
-    TORCH_CHECK(bias->dim() == 4 && (bias->size(0) == 1 || bias->size(0) == c.B) &&
-                    bias->size(1) == Hq && bias->size(2) == 1 && bias->size(3) >= max_len &&
-                    bias->scalar_type() == torch::kFloat && bias->stride(3) == 1 &&
-                    bias->device() == kc.device(),
-                "kv8_attn: bias must be fp32 (1 or B,Hq,1,>=max_len)");
-    a.bias = bias->data_ptr<float>();
-    a.bias_b = bias->size(0) > 1 ? bias->stride(0) : 0;
-    a.bias_h = bias->stride(1);
+    VALUE_CHECK(bias->dim() == 4 && (bias->size(0) == 1 || bias->size(0) == c.B) &&
+                    bias->size(1) == Hq && bias->size(2) == 1,
+                "decode_attention_kv8: bias ", bias->sizes(), " is not (1 or ", c.B, ", ", Hq, ", 1, .)");
+    const auto& m = mask(bias, 0, "bias");
+    a.bias = m.data_ptr<float>();
+    a.bias_b = m.size(0) > 1 ? m.stride(0) : 0;
+    a.bias_h = m.stride(1);
   }
   if (kpad.has_value() && kpad->defined()) {
-    TORCH_CHECK(kpad->dim() == 2 && kpad->size(0) == c.B && kpad->size(1) >= max_len &&
-                    kpad->scalar_type() == torch::kFloat && kpad->stride(1) == 1 &&
-                    kpad->device() == kc.device(),
-                "kv8_attn: kpad must be fp32 (B,>=max_len)");
-    a.kpad = kpad->data_ptr<float>();
-    a.kpad_b = kpad->stride(0);
+    VALUE_CHECK(kpad->dim() == 2 && kpad->size(0) == c.B,
+                "decode_attention_kv8: kpad ", kpad->sizes(), " is not (", c.B, ", .)");
+    const auto& m = mask(kpad, 1, "kpad");
+    a.kpad = m.data_ptr<float>();
+    a.kpad_b = m.stride(0);
   }
-  c10::DeviceGuard guard(kc.device());
   q = rows16(q);
-  auto out = torch::empty({c.B, Hq, 1, c.D}, q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto out = at::empty({c.B, Hq, 1, c.D}, q.options().memory_format(at::MemoryFormat::Contiguous));
   if (c.B == 0 || Hq == 0) return out;
   if (max_len == 0) return out.zero_();
   const int G = Hq / c.H;
@@ -751,7 +768,7 @@ torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torc
   const long nblk = (max_len + BLK - 1) / BLK;
   long nsplit = nblk < 32 ? 1 : std::max(1L, std::min({512 / (c.B * c.H * nz), nblk / 8, (long)MAX_SPLIT}));
   if (const char* ev = getenv("KV8_SPLIT")) nsplit = std::max(1L, std::min({atol(ev) / std::max(1L, c.B * c.H * nz), nblk / 4, (long)MAX_SPLIT}));
-  TORCH_CHECK(c.B * c.H < (1L << 31) && nz < 65536, "kv8_attn: too many heads");
+  VALUE_CHECK(nz < 65536, "decode_attention_kv8: too many heads");
   a.scale = (float)scale;
   a.share = nsplit > 1 || nblk > 3 ? 4 : nblk > 1 ? 2 : 1;
   a.BH = c.B * c.H; a.Hq = Hq; a.H = c.H; a.G = G; a.NB = c.NB; a.max_len = max_len; a.nsplit = nsplit;
@@ -781,8 +798,7 @@ torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torc
                          (int)nsplit);                                                           \
   } while (0)
   if (q.scalar_type() == torch::kBFloat16) BY_DIM(__hip_bfloat16, ATTN);
-  else if (q.scalar_type() == torch::kHalf) BY_DIM(__half, ATTN);
-  else TORCH_CHECK(false, "kv8_attn: bf16 or fp16 queries, got ", q.scalar_type());
+  else BY_DIM(__half, ATTN);
 #undef ATTN
 #undef BY_DIM
   HIP_CHECK_KERNEL();

@@ -743,28 +743,35 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
                             c10::optional<torch::Tensor> top_ks, long top_k,
                             c10::optional<torch::Tensor> top_ps, double top_p,
                             c10::optional<torch::Tensor> min_ps, double min_p, long empty_token) {
-  TORCH_CHECK(logits.dim() == 2 && logits.is_cuda(), "sample_tokens: logits must be (B,V) on a GPU");
+  NO_GRAD_CHECK(logits, "sample_tokens");
+  NO_GRAD_CHECK(u, "sample_tokens");
+  VALUE_CHECK(logits.dim() == 2 && logits.is_cuda() && logits.size(1) >= 1 && logits.size(1) <= MAX_V,
+              "sample_tokens: logits (B, V) with V from 1 to ", MAX_V, ", got ", logits.sizes());
   const long B = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V > 0 && V <= MAX_V, "sample_tokens: 1 to ", MAX_V, " logits a row, got ", V);
-  TORCH_CHECK(B < (1L << 31), "sample_tokens: too many rows");
-  TORCH_CHECK(u.dim() == 1 && u.size(0) == B && u.is_contiguous() &&
-                  u.device() == logits.device() &&
+  VALUE_CHECK(B < (1L << 31), "sample_tokens: too many rows");
+  VALUE_CHECK(u.dim() == 1 && u.size(0) == B && u.device() == logits.device() &&
                   (u.scalar_type() == torch::kFloat || u.scalar_type() == torch::kDouble),
-              "sample_tokens: u must be fp32 or fp64 (B,) on the logits' device");
-  auto opt = [&](const c10::optional<torch::Tensor>& each, double all, torch::ScalarType type,
-                 const char* what) -> Opt {
-    if (!each.has_value() || !each->defined()) return {nullptr, all};
-    TORCH_CHECK(each->dim() == 1 && each->size(0) == B && each->is_contiguous() &&
-                    each->scalar_type() == type && each->device() == logits.device(),
-                "sample_tokens: ", what, " must be a number or a ", type,
-                " (B,) tensor on the logits' device");
+              "sample_tokens: u must be fp32 or fp64 (", B, ",) on ", logits.device(), ", got ",
+              u.scalar_type(), " ", u.sizes(), " on ", u.device());
+  c10::DeviceGuard guard(logits.device());
+  if (!u.is_contiguous()) u = u.contiguous();
+  auto opt = [&](c10::optional<torch::Tensor>& each, double all, double least, double most,
+                 torch::ScalarType type, const char* what) -> Opt {
+    if (!each.has_value() || !each->defined()) {
+      VALUE_CHECK(all >= least && all <= most, "sampling: temperature and top_k are at least 0, "
+                  "top_p and min_p from 0 to 1; got ", what, " = ", all);
+      return {nullptr, all};
+    }
+    VALUE_CHECK(each->dim() == 1 && each->size(0) == B && each->device() == logits.device(),
+                "sample_tokens: ", what, " must be a number or a (", B, ",) tensor on ",
+                logits.device(), ", got ", each->sizes(), " on ", each->device());
+    if (each->scalar_type() != type || !each->is_contiguous()) each = each->to(type).contiguous();
     return {each->data_ptr(), all};
   };
-  const Opt ot = opt(temperatures, temperature, torch::kFloat, "temperature");
-  const Opt ok = opt(top_ks, (double)top_k, torch::kInt, "top_k");
-  const Opt op = opt(top_ps, top_p, torch::kFloat, "top_p");
-  const Opt om = opt(min_ps, min_p, torch::kFloat, "min_p");
-  c10::DeviceGuard guard(logits.device());
+  const Opt ot = opt(temperatures, temperature, 0.0, 1.7e308, torch::kFloat, "temperature");
+  const Opt ok = opt(top_ks, (double)std::min(top_k, V), 0.0, 1.7e308, torch::kInt, "top_k");
+  const Opt op = opt(top_ps, top_p, 0.0, 1.0, torch::kFloat, "top_p");
+  const Opt om = opt(min_ps, min_p, 0.0, 1.0, torch::kFloat, "min_p");
   auto out = torch::empty({B}, logits.options().dtype(torch::kLong));
   if (B == 0) return out;
   if (V < 8) logits = at::constant_pad_nd(logits, {0, 8 - V}, -INFINITY);   // a slot at least

@@ -393,25 +393,33 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 
 torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps,
                         torch::Tensor row_exp) {
-  TORCH_CHECK(x.dim() == 2 && codes.dim() == 2 && exps.dim() == 2 && row_exp.dim() == 1,
-              "w4_linear: x (M,K), codes (N,K/2), exps (N,K/32), row_exp (N)");
-  const long M = x.size(0), K = x.size(1), N = codes.size(0);
-  TORCH_CHECK(K > 0 && K % 32 == 0 && codes.size(1) * 2 == K && exps.size(0) == N &&
-                  exps.size(1) * 32 == K && row_exp.size(0) == N,
-              "w4_linear: x has ", K, " inputs, codes ", codes.size(1) * 2, ", exps ",
-              exps.size(1) * 32);
-  // a grid's second dimension is 16 bits wide: blocks of 16 rows, of 32 outputs
-  TORCH_CHECK(M < (1L << 31) - 256 && N < 65535L * 32 && K < (1L << 30), "w4_linear: too large");
-  for (const auto& t : {codes, exps, row_exp})
-    TORCH_CHECK(t.scalar_type() == torch::kByte && t.is_contiguous() && t.device() == x.device(),
-                "w4_linear: codes and exponents must be contiguous uint8 on x's device");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
-              "w4_linear: codes must be 16-byte aligned");
+  NO_GRAD_CHECK(x, "linear_w4");
+  VALUE_CHECK(codes.dim() == 2 && exps.dim() == 2 && row_exp.dim() == 1,
+              "linear_w4: codes (N,K/2), exps (N,K/32), row_exp (N)");
+  const long N = codes.size(0), K = 2 * codes.size(1);
+  VALUE_CHECK(x.dim() >= 1 && x.size(-1) == K && K > 0, "linear_w4: x ", x.sizes(),
+              ", the weight has ", K, " inputs");
+  VALUE_CHECK(K % 32 == 0 && exps.size(0) == N && exps.size(1) * 32 == K && row_exp.size(0) == N,
+              "linear_w4: codes ", codes.sizes(), " and exponents ", exps.sizes(), " do not match");
+  for (const auto* t : {&codes, &exps, &row_exp})
+    VALUE_CHECK(t->scalar_type() == torch::kByte && t->is_contiguous() && t->device() == x.device(),
+                "linear_w4: codes and exponents must be contiguous uint8 on x's device, ",
+                x.device(), ", got ", t->device());
+  VALUE_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
+              "linear_w4: codes must be 16-byte aligned");
+  VALUE_CHECK(x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kHalf,
+              "linear_w4 takes bf16 or fp16 on a GPU, got ", x.scalar_type());
   c10::DeviceGuard guard(x.device());
-  auto y = torch::empty({M, N}, x.options());
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  auto y = at::empty(sizes, x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (x.dim() != 2) x = x.reshape({-1, K});
+  const long M = x.size(0);
+  // a grid's second dimension is 16 bits wide: blocks of 16 rows, of 32 outputs
+  VALUE_CHECK(M < (1L << 31) - 256 && N < 65535L * 32 && K < (1L << 30), "linear_w4: too large");
   if (M == 0 || N == 0) return y;
   // rows of x are read 16 bytes at a time
-  if (x.stride(1) != 1 || x.stride(0) % 8 != 0 ||
+  if (x.stride(1) != 1 || (M > 1 && x.stride(0) % 8 != 0) ||
       reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0)
     x = x.clone(at::MemoryFormat::Contiguous);
   auto stream = at::hip::getCurrentHIPStream().stream();
@@ -476,8 +484,7 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
     else many(w4_many_rows<T, 2, 2, 2>, 2, 2, 2);
   };
   if (x.scalar_type() == torch::kBFloat16) go(__hip_bfloat16());
-  else if (x.scalar_type() == torch::kHalf) go(__half());
-  else TORCH_CHECK(false, "w4_linear: bf16 or fp16 inputs, got ", x.scalar_type());
+  else go(__half());
   HIP_CHECK_KERNEL();
   return y;
 }

@@ -5,6 +5,9 @@ All of it is inference only: weights and caches are codes and tokens are whole
 numbers, so inputs that ask for a gradient are refused.  On a GPU tensor the
 hand-written kernels run (``csrc/kernels/{w4_linear,kv8,sample}.hip``); CPU
 tensors take the plain-PyTorch forms in ``torch_ref``.
+
+Calls here are a few microseconds on the GPU, so the GPU path goes straight to
+the extension, which checks the arguments (ValueError, as on the CPU path).
 """
 from __future__ import annotations
 
@@ -13,9 +16,6 @@ import math
 import torch
 
 from . import _load_ext, _use_hip, torch_ref
-
-_LOWP = (torch.bfloat16, torch.float16)
-
 
 def _no_grad(what: str, *tensors):
     if torch.is_grad_enabled():
@@ -94,18 +94,15 @@ def quantize_w4(weight: torch.Tensor) -> W4Weight:
 def linear_w4(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     """``x @ w.T`` for x (..., K) in bf16 or fp16: sums in 32 bits, one rounding
     at the end.  Any number of rows; made for the few that decoding has."""
-    n, k = w.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"linear_w4: x has {x.shape[-1]} inputs, the weight {k}")
+    if x.is_cuda and _use_hip(x):
+        b = w._buffers
+        return _load_ext().w4_linear(x, b["codes"], b["exps"], b["row_exp"])
     _no_grad("linear_w4", x)
+    if x.dim() == 0 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"linear_w4: x {tuple(x.shape)}, the weight has {w.shape[1]} inputs")
     if w.codes.device != x.device:
         raise ValueError(f"linear_w4: x on {x.device}, the weight on {w.codes.device}")
-    if not x.is_cuda or not _use_hip(x):
-        return torch_ref.linear_w4(x, w.codes, w.exps)
-    if x.dtype not in _LOWP:
-        raise ValueError(f"linear_w4 takes bf16 or fp16 on a GPU, got {x.dtype}")
-    y = _load_ext().w4_linear(x if x.dim() == 2 else x.reshape(-1, k), w.codes, w.exps, w.row_exp)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+    return torch_ref.linear_w4(x, w.codes, w.exps)
 
 
 # --------------------------------------------------------------------------- #
@@ -170,6 +167,13 @@ def kv8_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start, counts=
     tensor, those past the capacity are not written, and a negative one skips
     the sequence.  Infinities saturate and do not widen a scale; NaN stays NaN.
     """
+    if counts is not None and not torch.is_tensor(counts):
+        raise ValueError("kv8_append: counts is an int32 (B,) tensor")
+    if k.is_cuda and _use_hip(k):
+        each = torch.is_tensor(start)
+        _load_ext().kv8_append(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                               start if each else None, 0 if each else start, counts)
+        return
     _no_grad("kv8_append", k, v)
     b, h, cap, d = cache.k.shape
     if k.dim() != 4 or k.shape != v.shape or k.shape[:2] != (b, h) or k.shape[3] != d or k.dtype != v.dtype:
@@ -181,16 +185,9 @@ def kv8_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start, counts=
     if starts is None and (start < 0 or start + k.shape[2] > cap):
         raise ValueError(f"kv8_append: {k.shape[2]} tokens at {start} do not fit a cache of {cap}")
     if counts is not None:
-        if not torch.is_tensor(counts):
-            raise ValueError("kv8_append: counts is an int32 (B,) tensor")
         counts, _ = _per_row(counts, "counts", b, k.device, torch.int32)
-    if not k.is_cuda or not _use_hip(k):
-        torch_ref.kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v,
-                             start if starts is None else starts, counts)
-        return
-    if k.dtype not in _LOWP:
-        raise ValueError(f"kv8_append takes bf16 or fp16 on a GPU, got {k.dtype}")
-    _load_ext().kv8_append(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale, starts, start, counts)
+    torch_ref.kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v,
+                         start if starts is None else starts, counts)
 
 
 def decode_attention_kv8(q: torch.Tensor, cache: KVCache8, lengths, bias=None, kpad=None,
@@ -205,6 +202,11 @@ def decode_attention_kv8(q: torch.Tensor, cache: KVCache8, lengths, bias=None, k
     with -inf is not there, whatever it holds.  A row without keys is 0.
     Scores are ``scale * q.k + bias + kpad``, in fp32 as are the sums.
     """
+    if q.is_cuda and _use_hip(q):
+        each = torch.is_tensor(lengths)
+        return _load_ext().kv8_attn(q, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                    lengths if each else None, 0 if each else lengths,
+                                    -1 if max_len is None else max_len, max_len is not None, bias, kpad, scale)
     _no_grad("decode_attention_kv8", q, bias, kpad)
     b, h, cap, d = cache.k.shape
     if q.dim() != 4 or q.shape[0] != b or q.shape[2] != 1 or q.shape[3] != d or not h or q.shape[1] % h:
@@ -228,17 +230,8 @@ def decode_attention_kv8(q: torch.Tensor, cache: KVCache8, lengths, bias=None, k
                              or kpad.device != q.device):
         raise ValueError(f"decode_attention_kv8: kpad {tuple(kpad.shape)} on {kpad.device} is not "
                          f"({b}, >= {max_len})")
-    if not q.is_cuda or not _use_hip(q):
-        return torch_ref.decode_attention_kv8(q, cache.k, cache.v, cache.k_scale, cache.v_scale,
-                                              length if each is None else each, bias, kpad, scale, max_len)
-    if q.dtype not in _LOWP:
-        raise ValueError(f"decode_attention_kv8 takes bf16 or fp16 on a GPU, got {q.dtype}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.stride(3) != 1):
-        bias = bias.float().contiguous()
-    if kpad is not None and (kpad.dtype != torch.float32 or kpad.stride(1) != 1):
-        kpad = kpad.float().contiguous()
-    return _load_ext().kv8_attn(q, cache.k, cache.v, cache.k_scale, cache.v_scale, each, length,
-                                max_len, bias, kpad, scale)
+    return torch_ref.decode_attention_kv8(q, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                          length if each is None else each, bias, kpad, scale, max_len)
 
 
 # --------------------------------------------------------------------------- #
@@ -267,6 +260,13 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     ``empty_token``.  Weights under 2^-45 of the largest count as 0.
     Returns int64 (B,).
     """
+    if logits.is_cuda and _use_hip(logits):
+        is_t = torch.is_tensor
+        t, k, p, m = is_t(temperature), is_t(top_k), is_t(top_p), is_t(min_p)
+        return _load_ext().sample_tokens(
+            logits, u, temperature if t else None, 1.0 if t else temperature,
+            top_k if k else None, 0 if k else top_k, top_p if p else None, 1.0 if p else top_p,
+            min_p if m else None, 0.0 if m else min_p, empty_token)
     if logits.dim() != 2 or not 1 <= logits.shape[1] <= 1 << 19:
         raise ValueError(f"sample_tokens: logits (B, V) with V from 1 to {1 << 19}, got {tuple(logits.shape)}")
     if u.shape != logits.shape[:1] or u.device != logits.device or u.dtype not in (torch.float32, torch.float64):
@@ -279,10 +279,6 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     ps, top_p = _per_row(top_p, "top_p", rows, dev, torch.float32)
     mins, min_p = _per_row(min_p, "min_p", rows, dev, torch.float32)
     check_sampling(temperature, top_k, top_p, min_p)
-    top_k = min(top_k, logits.shape[1])
-    if not logits.is_cuda or not _use_hip(logits):
-        pick = lambda each, one: one if each is None else each  # noqa: E731
-        return torch_ref.sample_tokens(logits, u, pick(temps, temperature), pick(ks, top_k),
-                                       pick(ps, top_p), pick(mins, min_p), empty_token)
-    return _load_ext().sample_tokens(logits, u.contiguous(), temps, temperature, ks, top_k, ps, top_p,
-                                     mins, min_p, empty_token)
+    pick = lambda each, one: one if each is None else each  # noqa: E731
+    return torch_ref.sample_tokens(logits, u, pick(temps, temperature), pick(ks, top_k), pick(ps, top_p),
+                                   pick(mins, min_p), empty_token)
