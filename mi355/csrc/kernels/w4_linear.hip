@@ -79,19 +79,49 @@ struct Args {
   long ldx;
 };
 
+// The block's waves hold sums over parts of K, each for the 16 * NT outputs from
+// n0 - lane%16 on: added through LDS in wave order (the same sum every time) and
+// stored.  D layout: column n = lane%16, row m = 4*(lane/16) + r.
+template <typename T, int NT, int WAVES>
+DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, T* y, const Args& a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) part[wave][u][lane] = acc[u];
+  __syncthreads();
+  for (int u = wave; u < NT; u += WAVES) {
+    const int n = n0 + 16 * u;
+    f32x4 s = part[0][u][lane];
+#pragma unroll
+    for (int v = 1; v < WAVES; ++v) {
+      const f32x4 p = part[v][u][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += p[r];
+    }
+    if (n >= a.N) continue;
+    const float back = row_scale(a.row_exp[n]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = 4 * (lane >> 4) + r;
+      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Up to 16*MT rows, x straight from the caches: one wave owns 16*NT outputs
-// and every WAVES-th 128-wide piece of K, the next piece's weights and x on
-// their way while this one is multiplied.  The block's waves are summed through
-// LDS in wave order (the same sum every time).
+// Up to 16 rows, x straight from the caches: one wave owns 16*NT outputs and
+// every WAVES-th 128-wide piece of K, the next piece's weights and x on their
+// way while this one is multiplied.  NT tiles of outputs share a wave's x: 16
+// rows by 10240 x 2048 take 8.1 us with four of them, 10.6 with one; 16 rows by
+// 2304 x 768, too few outputs for that, 3.8 and 3.1 us.
 // ---------------------------------------------------------------------------
-template <typename T, int MT, int NT, int WAVES>
+template <typename T, int NT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   using vec = typename Frag<T>::vec;
+  __shared__ f32x4 part[WAVES][NT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
-  const int n0 = blockIdx.x * (16 * NT) + c16, m0 = blockIdx.y * (16 * MT) + c16;
+  const int n0 = blockIdx.x * (16 * NT) + c16;
   int row_e[NT];
   const unsigned char *crow[NT], *erow[NT];
 #pragma unroll
@@ -103,7 +133,7 @@ w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   }
 
   struct Piece {
-    u32x4 w[NT], x[MT][4];
+    u32x4 w[NT], x[4];
     int e[NT];
   };
   auto load = [&](int k0) {
@@ -120,22 +150,16 @@ w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
       }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p.x[t][i] = u32x4{0u, 0u, 0u, 0u};
-        if (k_ok && m0 + 16 * t < a.M)
-          p.x[t][i] = *reinterpret_cast<const u32x4*>(x + (m0 + 16 * t) * a.ldx + k + 8 * i);
-      }
+    for (int i = 0; i < 4; ++i) {
+      p.x[i] = u32x4{0u, 0u, 0u, 0u};
+      if (k_ok && c16 < a.M) p.x[i] = *reinterpret_cast<const u32x4*>(x + c16 * a.ldx + k + 8 * i);
+    }
     return p;
   };
 
-  f32x4 acc[MT][NT];
+  f32x4 acc[NT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+  for (int u = 0; u < NT; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
   Piece next = load(wave * 128);
   for (int k0 = wave * 128; k0 < a.K; k0 += WAVES * 128) {
     const Piece p = next;
@@ -144,46 +168,25 @@ w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     for (int u = 0; u < NT; ++u) {
       const float scale = group_scale(p.e[u], row_e[u]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const vec wf = decode8<T>(p.w[u][i], scale);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          acc[t][u] = Frag<T>::mfma(__builtin_bit_cast(vec, p.x[t][i]), wf, acc[t][u]);
-      }
+      for (int i = 0; i < 4; ++i)
+        acc[u] = Frag<T>::mfma(__builtin_bit_cast(vec, p.x[i]), decode8<T>(p.w[u][i], scale), acc[u]);
     }
   }
-
-  __shared__ f32x4 part[WAVES][MT * NT][64];
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int u = 0; u < NT; ++u) part[wave][t * NT + u][lane] = acc[t][u];
-  __syncthreads();
-  // D layout: column n = lane%16, row m = 4*(lane/16) + r
-  for (int q = wave; q < MT * NT; q += WAVES) {
-    const int t = q / NT, n = n0 + 16 * (q % NT);
-    f32x4 s = part[0][q][lane];
-#pragma unroll
-    for (int v = 1; v < WAVES; ++v) {
-      const f32x4 p = part[v][q][lane];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] += p[r];
-    }
-    if (n >= a.N) continue;
-    const float back = row_scale(a.row_exp[n]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = m0 - c16 + 16 * t + 4 * g + r;
-      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
-    }
-  }
+  add_waves<T, NT, WAVES>(part, acc, n0, y, a);
 }
 
-// Up to 16 rows of x in LDS.
+// The same with x in LDS, for few enough rows that a workgroup's copy is small
+// beside its weights: of the 64 lanes that the matrix instruction has for x only
+// M in 16 hold a row (the others repeat the last; their sums are not stored),
+// and fetching those from the caches takes as many memory instructions as the
+// weights.  U pieces of 128 lie next to each other.  One row by 20480 x 4096:
+// 12.7 us (3.5 TB/s of weights) here with 4 waves of two pieces, 13.5 with 8 of
+// one, 17 with x from the caches; 16 rows by 10240 x 2048 11 against 8.1.
 template <typename T, int NT, int U, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   using vec = typename Frag<T>::vec;
+  __shared__ f32x4 part[WAVES][NT][64];
   extern __shared__ char shared[];
   T* xs = reinterpret_cast<T*>(shared);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -249,35 +252,19 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
       }
     }
   }
-  __shared__ f32x4 part[WAVES][NT][64];
-#pragma unroll
-  for (int u = 0; u < NT; ++u) part[wave][u][lane] = acc[u];
-  __syncthreads();
-  for (int q = wave; q < NT; q += WAVES) {
-    const int n = n0 + 16 * q;
-    f32x4 s = part[0][q][lane];
-#pragma unroll
-    for (int v = 1; v < WAVES; ++v) {
-      const f32x4 p = part[v][q][lane];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] += p[r];
-    }
-    if (n >= a.N) continue;
-    const float back = row_scale(a.row_exp[n]);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int m = 4 * g + r;
-      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
-    }
-  }
+  add_waves<T, NT, WAVES>(part, acc, n0, y, a);
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup of 2 x 2 waves makes 2*16*MT rows by 2*16*NT outputs.
+// Many rows: a workgroup of 2 x WN waves makes 32*MT rows by 16*NT*WN outputs.
 // x goes through LDS, 128 of K at a time in two buffers (two pieces are on
-// their way in registers while one is multiplied, rows 16 bytes apart from a
-// multiple of 256 so that 16 rows at one k lie in different banks); weights
+// their way in registers while one is multiplied; rows lie 16 bytes apart from
+// a multiple of 256, so that 16 rows at one k are in different banks); weights
 // go from memory to registers as above, converted once for MT tiles of rows.
+// Tiles of 128 x 128 once there are 128 of them for the 256 CUs, else of
+// 64 x 64 once there are 128, else of 32 x 32: 256 rows by 10240 x 2048 take
+// 27, 33 and 52 us, by 4096 x 768 13, 6.4 and 9.2 us, by 768 x 2048 25, 12 and
+// 7.6 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).
 // ---------------------------------------------------------------------------
 template <typename T, int MT, int NT, int WN>
 __global__ void __launch_bounds__(128 * WN)
@@ -299,35 +286,35 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     crow[t] = a.codes + (long)n * (a.K >> 1);
     erow[t] = a.exps + (long)n * (a.K >> 5);
   }
+  // Loads carry no condition, so that the compiler can count them and wait for
+  // no younger ones: addresses are clamped, what they are clamped for becomes 0
+  // where it is used.
   struct Piece {
     u32x4 x[LOADS], w[NT];
     int e[NT];
   } ahead[2];
-  auto load = [&](Piece& p, int k0) {
+  const T* xrow[LOADS];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int piece = threadIdx.x + THREADS * i;
-      const int m = m_at + piece / (KC / 8), k = k0 + piece % (KC / 8) * 8;
-      p.x[i] = u32x4{0u, 0u, 0u, 0u};
-      if (m < a.M && k < a.K) p.x[i] = *reinterpret_cast<const u32x4*>(x + m * a.ldx + k);
-    }
-    const int k = k0 + 32 * g;                    // K is a multiple of 32
+  for (int i = 0; i < LOADS; ++i)
+    xrow[i] = x + min(m_at + (int)(threadIdx.x + THREADS * i) / (KC / 8), a.M - 1) * a.ldx;
+  const int xk = threadIdx.x % (KC / 8) * 8;        // the same k for all of a thread's pieces
+  static_assert(THREADS % (KC / 8) == 0, "");
+  auto load = [&](Piece& p, int k0) {
+    const int k = min(k0 + xk, a.K - 8);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) p.x[i] = *reinterpret_cast<const u32x4*>(xrow[i] + k);
+    const int kk = min(k0 + 32 * g, a.K - 32);      // K is a multiple of 32
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      p.w[t] = u32x4{0u, 0u, 0u, 0u};
-      p.e[t] = 127;
-      if (k < a.K) {
-        p.w[t] = *reinterpret_cast<const u32x4*>(crow[t] + (k >> 1));
-        p.e[t] = erow[t][k >> 5];
-      }
+      p.w[t] = *reinterpret_cast<const u32x4*>(crow[t] + (kk >> 1));
+      p.e[t] = erow[t][kk >> 5];
     }
   };
-  auto stage = [&](const Piece& p, int buf) {
+  auto stage = [&](const Piece& p, int k0, int buf) {
+    const unsigned keep = k0 + xk < a.K ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int piece = threadIdx.x + THREADS * i;
-      *reinterpret_cast<u32x4*>(&lds[buf][piece / (KC / 8) * LD + piece % (KC / 8) * 8]) = p.x[i];
-    }
+    for (int i = 0; i < LOADS; ++i)
+      *reinterpret_cast<u32x4*>(&lds[buf][(threadIdx.x + THREADS * i) / (KC / 8) * LD + xk]) = p.x[i] & keep;
   };
   // orders LDS alone: a plain barrier would wait for the loads on their way
   auto lds_barrier = [] {
@@ -345,11 +332,12 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   // multiplies the piece in `buf`, whose weights are in `now`, while that after
   // the next is loaded
   auto step = [&](int k0, Piece& now, const Piece& next, int buf) {
+    const unsigned keep = k0 + 32 * g < a.K ? 0xffffffffu : 0u;
     u32x4 w[NT];
     float scale[NT];
 #pragma unroll
-    for (int u = 0; u < NT; ++u) { w[u] = now.w[u]; scale[u] = group_scale(now.e[u], row_e[u]); }
-    if (k0 + 2 * KC < a.K) load(now, k0 + 2 * KC);
+    for (int u = 0; u < NT; ++u) { w[u] = now.w[u] & keep; scale[u] = group_scale(now.e[u], row_e[u]); }
+    load(now, k0 + 2 * KC);
     const T* row = &lds[buf][(wm * 16 * MT + c16) * LD + 32 * g];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -363,16 +351,17 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
         for (int t = 0; t < MT; ++t) acc[t][u] = Frag<T>::mfma(xf[t], wf, acc[t][u]);
       }
     }
-    if (k0 + KC < a.K) stage(next, buf ^ 1);
+    stage(next, k0 + KC, buf ^ 1);
     lds_barrier();
   };
   load(ahead[0], 0);
-  if (KC < a.K) load(ahead[1], KC);
-  stage(ahead[0], 0);
+  load(ahead[1], KC);
+  stage(ahead[0], 0, 0);
   lds_barrier();
+  // in pairs; of an odd number of pieces the last is multiplied by zeros
   for (int k0 = 0; k0 < a.K; k0 += 2 * KC) {
     step(k0, ahead[0], ahead[1], 0);
-    if (k0 + KC < a.K) step(k0 + KC, ahead[1], ahead[0], 1);
+    step(k0 + KC, ahead[1], ahead[0], 1);
   }
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
@@ -425,63 +414,30 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
   auto stream = at::hip::getCurrentHIPStream().stream();
   const Args a{codes.data_ptr<unsigned char>(), exps.data_ptr<unsigned char>(),
                row_exp.data_ptr<unsigned char>(), (int)M, (int)N, (int)K, (long)x.stride(0)};
-  const char* ev = getenv("W4_CFG");
-  const int cfg = ev ? atoi(ev) : 0;
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    auto few = [&](auto kernel, int mt, int nt, int waves) {
-      hipLaunchKernelGGL(kernel, dim3((N + 16 * nt - 1) / (16 * nt), (M + 16 * mt - 1) / (16 * mt)),
-                         dim3(waves * 64), 0, stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
+    auto launch = [&](auto kernel, dim3 grid, int threads, long lds) {
+      hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, stream, (const T*)x.data_ptr(),
+                         (T*)y.data_ptr(), a);
     };
-    auto many = [&](auto kernel, int mt, int nt, int wn) {
-      hipLaunchKernelGGL(kernel, dim3((M + 32 * mt - 1) / (32 * mt), (N + 16 * nt * wn - 1) / (16 * nt * wn)),
-                         dim3(128 * wn), 0, stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
-    };
-    auto lds = [&](auto kernel, int nt, int waves) {
-      hipLaunchKernelGGL(kernel, dim3((N + 16 * nt - 1) / (16 * nt)), dim3(waves * 64), M * (K + 8) * 2,
-                         stream, (const T*)x.data_ptr(), (T*)y.data_ptr(), a);
-    };
-    switch (cfg) {
-      case 21: lds(w4_lds_rows<T, 1, 1, 8>, 1, 8); return;
-      case 22: lds(w4_lds_rows<T, 1, 2, 8>, 1, 8); return;
-      case 23: lds(w4_lds_rows<T, 1, 4, 8>, 1, 8); return;
-      case 24: lds(w4_lds_rows<T, 1, 1, 16>, 1, 16); return;
-      case 25: lds(w4_lds_rows<T, 1, 2, 16>, 1, 16); return;
-      case 26: lds(w4_lds_rows<T, 2, 1, 8>, 2, 8); return;
-      case 27: lds(w4_lds_rows<T, 2, 2, 8>, 2, 8); return;
-      case 28: lds(w4_lds_rows<T, 1, 2, 4>, 1, 4); return;
-      case 29: lds(w4_lds_rows<T, 1, 4, 4>, 1, 4); return;
-      case 30: lds(w4_lds_rows<T, 2, 2, 4>, 2, 4); return;
-      case 31: lds(w4_lds_rows<T, 2, 4, 4>, 2, 4); return;
-      case 32: lds(w4_lds_rows<T, 2, 2, 16>, 2, 16); return;
-      case 1: few(w4_few_rows<T, 1, 1, 8>, 1, 1, 8); return;
-      case 2: few(w4_few_rows<T, 1, 2, 8>, 1, 2, 8); return;
-      case 3: few(w4_few_rows<T, 1, 4, 8>, 1, 4, 8); return;
-      case 4: few(w4_few_rows<T, 1, 2, 4>, 1, 2, 4); return;
-      case 5: few(w4_few_rows<T, 1, 4, 4>, 1, 4, 4); return;
-      case 6: few(w4_few_rows<T, 2, 2, 4>, 2, 2, 4); return;
-      case 7: few(w4_few_rows<T, 2, 1, 8>, 2, 1, 8); return;
-      case 8: few(w4_few_rows<T, 4, 1, 4>, 4, 1, 4); return;
-      case 9: few(w4_few_rows<T, 2, 4, 4>, 2, 4, 4); return;
-      case 10: few(w4_few_rows<T, 1, 1, 4>, 1, 1, 4); return;
-      case 11: many(w4_many_rows<T, 1, 1, 2>, 1, 1, 2); return;
-      case 12: many(w4_many_rows<T, 2, 2, 2>, 2, 2, 2); return;
-      case 13: many(w4_many_rows<T, 4, 2, 2>, 4, 2, 2); return;
-      case 14: many(w4_many_rows<T, 2, 4, 2>, 2, 4, 2); return;
-      case 15: many(w4_many_rows<T, 4, 4, 2>, 4, 4, 2); return;
-      case 16: many(w4_many_rows<T, 1, 2, 2>, 1, 2, 2); return;
-      case 17: many(w4_many_rows<T, 2, 1, 2>, 2, 1, 2); return;
-      case 18: many(w4_many_rows<T, 4, 1, 2>, 4, 1, 2); return;
-      case 41: many(w4_many_rows<T, 4, 2, 4>, 4, 2, 4); return;
-      case 42: many(w4_many_rows<T, 4, 1, 4>, 4, 1, 4); return;
-      case 43: many(w4_many_rows<T, 2, 2, 4>, 2, 2, 4); return;
-      case 44: many(w4_many_rows<T, 2, 1, 4>, 2, 1, 4); return;
-      case 45: many(w4_many_rows<T, 4, 4, 4>, 4, 4, 4); return;
-      case 46: many(w4_many_rows<T, 1, 1, 4>, 1, 1, 4); return;
-      case 47: many(w4_many_rows<T, 1, 2, 4>, 1, 2, 4); return;
+    const auto up = [](long n, long by) { return (n + by - 1) / by; };
+    const auto tiles = [&](long t) { return dim3(up(M, t), up(N, t)); };
+    const auto count = [](dim3 d) { return (long)d.x * d.y; };
+    const long copy = M * (K + 8) * 2;              // x in LDS
+    if (M <= 8 && copy <= 56 * 1024) {
+      if (M <= 2 && N >= 16384) launch(w4_lds_rows<T, 1, 2, 4>, dim3(up(N, 16)), 256, copy);
+      else launch(w4_lds_rows<T, 1, 1, 8>, dim3(up(N, 16)), 512, copy);
+    } else if (M <= 16) {
+      if (N < 8192) launch(w4_few_rows<T, 1, 8>, dim3(up(N, 16)), 512, 0);
+      else if (M <= 8) launch(w4_few_rows<T, 2, 8>, dim3(up(N, 32)), 512, 0);
+      else launch(w4_few_rows<T, 4, 8>, dim3(up(N, 64)), 512, 0);
+    } else if (count(tiles(128)) >= 128) {
+      launch(w4_many_rows<T, 4, 2, 4>, tiles(128), 512, 0);
+    } else if (count(tiles(64)) >= 128) {
+      launch(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, 0);
+    } else {
+      launch(w4_many_rows<T, 1, 1, 2>, tiles(32), 256, 0);
     }
-    if (M <= 16) few(w4_few_rows<T, 1, 1, 8>, 1, 1, 8);
-    else many(w4_many_rows<T, 2, 2, 2>, 2, 2, 2);
   };
   if (x.scalar_type() == torch::kBFloat16) go(__hip_bfloat16());
   else go(__half());
