@@ -213,7 +213,7 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
                       int BH, int H, int NB) {
   constexpr int PER = D > 64 ? D / 64 : 1;        // values a lane holds
   const int lane = threadIdx.x & 63;
-  const int bh = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int bh = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool is_v = blockIdx.y;
   if (bh >= BH) return;
   const int b = bh / H, h = bh % H;
@@ -346,7 +346,7 @@ struct AttnArgs {
   long bias_b, bias_h, kpad_b;
   float scale;
   int BH, Hq, H, G, NB, max_len, nsplit;
-  int share;           // waves that share a sequence and head: 1, 2 or 4 of a workgroup's 4
+  int share;           // waves of a workgroup's 4 that share a sequence and head: 1, 2 or 4
 };
 
 constexpr int MAX_SPLIT = 256;
@@ -374,7 +374,8 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
   constexpr int WAVES = 4;
   constexpr int KSTEP = D / 32;        // matrix instructions along d
   constexpr int DT16 = D / 16;         // tiles of 16 d
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // known to be uniform
   const int g = lane >> 4, c16 = lane & 15;
   const int sub = wave & (a.share - 1);                // of the waves that share
   const long bh_at = (long)blockIdx.x * (WAVES / a.share) + wave / a.share;
@@ -411,7 +412,16 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
     const unsigned char* vb = vc + (bh * a.NB + blk) * (long)(BLK * D);
     const float kscale = ksc[bh * a.NB + blk] * a.scale;
     const float vscale = vsc[bh * a.NB + blk];
-    // loads first: V's are in flight while the scores are made
+    const int tok0 = blk * BLK + 16 * g;               // this lane group's 16 tokens
+    const int tok = tok0 + part16 * GP;                // this lane's GP of them
+    float add[GP], pad[GP];
+#pragma unroll
+    for (int i = 0; i < GP; ++i) {
+      const int at = min(tok + i, len - 1);
+      add[i] = bias ? bias[at] : 0.f;
+      pad[i] = kpad ? kpad[at] : 0.f;
+    }
+    // loads in the order of their use: V's are in flight while scores are made
     u32x2 kr[4][KSTEP];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -422,16 +432,6 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
 #pragma unroll
     for (int i = 0; i < DT16; ++i)
       vr[i] = *reinterpret_cast<const u32x4*>(vb + (16 * i + c16) * BLK + 16 * g);
-    const int tok0 = blk * BLK + 16 * g;               // this lane group's 16 tokens
-    const int tok = tok0 + part16 * GP;                // this lane's GP of them
-    float add[GP], pad[GP];
-#pragma unroll
-    for (int i = 0; i < GP; ++i) {
-      const int at = min(tok + i, len - 1);
-      add[i] = bias ? bias[at] : 0.f;
-      pad[i] = kpad ? kpad[at] : 0.f;
-    }
-
     f32x16 sc;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -552,11 +552,10 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
     if (g == 0) { sm[wave][c16] = m; sl[wave][c16] = l; }
   }
   __syncthreads();
-  const int ncol = min(GP, a.G - q0);
-  for (int e = threadIdx.x; e < WAVES / a.share * ncol * D; e += 256) {
-    const int d = e % D, c = e / D % ncol, w0 = e / D / ncol * a.share;
-    const long row = (long)blockIdx.x * (WAVES / a.share) + w0 / a.share;
-    if (row >= a.BH) break;
+  for (int e = threadIdx.x; e < WAVES / a.share * GP * D; e += 256) {
+    const int d = e % D, c = e / D % GP, pair = e / D / GP, w0 = pair * a.share;
+    const long row = (long)blockIdx.x * (WAVES / a.share) + pair;
+    if (row >= a.BH || q0 + c >= a.G) continue;
     float mm = -INFINITY;
     for (int w = w0; w < w0 + a.share; ++w) mm = fmaxf(mm, sm[w][c]);
     const float ref = mm == -INFINITY ? 0.f : mm;

@@ -85,11 +85,11 @@ DEVINL int index_of(u64 key) { return (int)~(unsigned)key; }
 // 2^(y/32) = 2^(n/32) * e^(f ln2/32) with |f| <= 1/2.
 struct Weights {
   double max, slope;
-  float least;         // whose weight is under 2^-46: taken for what is less, and for NaN
   const u64* table;
   // the integer in the low 52 bits, under the exponent field of 2^52
   DEVINL u64 raw(float x) const {
-    const double y = ((double)fmaxf(x, least) - max) * slope;
+    // what is under 2^-46, and NaN, becomes 2^-47 here and 0 in the integer
+    const double y = fmax(((double)x - max) * slope, -47.0 * TABLE);
     // added to 1.5 * 2^52, y is rounded to the integer in the low bits
     const double magic = 6755399441055744.0;
     const double rounded = y + magic;
@@ -373,6 +373,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   float mn = -wave_reduce_max(mine > -INFINITY ? -mine : -INFINITY);
   if (lane == 0) { s.red[0][wave] = mx; s.red[1][wave] = mn; }
   double temp = temperature.f(r);
+  temp = temp > 1e30 ? 1e30 : temp;                 // infinity among a row's options
   const int k = top_k.i(r);
   const double p = top_p.f(r);
   double floor_p = min_p.f(r);
@@ -399,9 +400,8 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   }
 
   const double slope = 46.16624130844683 / temp;
-  // 48 * 32 / slope below the maximum, or a rounding of it: over 2^-46.5 away
-  const Weights weight{(double)mx, slope, mx - (float)(48.0 * TABLE / slope), s.table};
-  floor_p = floor_p < 1.0 ? floor_p : 1.0;          // the maximum always stays
+  const Weights weight{(double)mx, slope, s.table};
+  floor_p = floor_p > 1.0 ? 1.0 : floor_p;          // the maximum always stays
   const u64 min_w = floor_p > 0.0 ? (u64)__builtin_rint(floor_p * ONE) : 0;
 
   // Bins over the distance from the maximum that matters: the spread of the

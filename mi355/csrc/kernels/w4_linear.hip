@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(WAVES * 64)
 w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   using vec = typename Frag<T>::vec;
   __shared__ f32x4 part[WAVES][NT][64];
-  extern __shared__ char shared[];
+  extern __shared__ u32x4 shared[];
   T* xs = reinterpret_cast<T*>(shared);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;

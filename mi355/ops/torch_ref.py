@@ -264,6 +264,7 @@ def sample_tokens(logits, u, temperature, top_k, top_p, min_p, empty_token: int 
             torch.full((len(x), 1), v, device=x.device, dtype=dtype)
 
     t, k = column(temperature, torch.float64), column(top_k, torch.int64)
+    t = t.clamp(max=1e30)
     p, floor = column(top_p, torch.float64), column(min_p, torch.float64).clamp(max=1.0)
     greedy = ~(t > 0)
     k = torch.where(greedy, 1, torch.where(k <= 0, x.shape[1], k))
@@ -279,7 +280,7 @@ def sample_tokens(logits, u, temperature, top_k, top_p, min_p, empty_token: int 
     keep = (rank < k) & ((rank == 0) | ~(p < 1) | (before < p * cum[:, -1:])) & ~(ws < floor)
     kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, ws, 0.0))
     cum = kept.cumsum(1)
-    r = u.double().clamp(min=0.0)[:, None] * cum[:, -1:]
+    r = u.double().nan_to_num(0.0).clamp(min=0.0)[:, None] * cum[:, -1:]
     over = (cum > r) & (kept > 0)
     # u = 1 (or a rounding of u times the sum): the last one kept
     ids = torch.where(over.any(1), over.to(torch.int8).argmax(1),

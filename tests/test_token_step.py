@@ -424,6 +424,31 @@ def test_decode_attention_kv8_max_len(device):
         check_attention(q, cache, lengths, None, None, 1.0, out, max_len=min(max_len or 256, 256))
 
 
+@gpu
+def test_kv8_offsets_over_32_bits():
+    """Heads whose codes begin 4.3 GB into the cache."""
+    cache = ops.KVCache8(1, 34, 1 << 20, 128, device="cuda")
+    k, v, q = (tokens(1, 34, n, 128, j, "cuda", BF16) for j, n in ((1, 200), (2, 200), (3, 1)))
+    at = (1 << 20) - 200
+    for start in (0, at):
+        ops.kv8_append(cache, k[:, :, :199], v[:, :, :199], start)
+        ops.kv8_append(cache, k[:, :, 199:], v[:, :, 199:], start + 199)
+    small = ops.KVCache8(1, 34, 256, 128, device="cuda")
+    ops.kv8_append(small, k, v, 0)
+    assert torch.equal(ops.decode_attention_kv8(q, cache, 200), ops.decode_attention_kv8(q, small, 200))
+    # of the whole cache all but the last 200 tokens are masked
+    kpad = torch.full((1, 1 << 20), -math.inf, device="cuda")
+    kpad[:, at:] = 0
+    out = ops.decode_attention_kv8(q, cache, 1 << 20, kpad=kpad, scale=0.1)
+    part = ops.KVCache8(1, 34, 256, 128, device="cuda")
+    first = at // 64 * 64
+    part.k[:, :, :(1 << 20) - first] = cache.k[:, :, first:]
+    n = ((1 << 20) - first) // 64
+    part.v[:, :, :n], part.k_scale[:, :, :n], part.v_scale[:, :, :n] = (
+        cache.v[:, :, -n:], cache.k_scale[:, :, -n:], cache.v_scale[:, :, -n:])
+    check_attention(q, part, (1 << 20) - first, None, kpad[:, first:], 0.1, out)
+
+
 # --------------------------------------------------------------------------- #
 # sampling                                                                    #
 # --------------------------------------------------------------------------- #
@@ -538,6 +563,48 @@ def test_sample_tokens_per_row_and_strides(device):
         got = ops.sample_tokens(logits, u, temperature=t, top_k=k.long(), top_p=p, min_p=m)
         assert got.tolist() == sample_by_definition(logits, u, t, k, p.clamp(0, 1), m)
     assert ops.sample_tokens(base[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_tokens_odd_options(device):
+    """Temperatures so small that all weight is the maximum's and so large that
+    none is less than another's, infinite and NaN options of a row, NaN as u."""
+    logits = randn(6, 3001, seed=101, device=device) * 3 + 20
+    u = uniform(6, 102, device)
+    best = logits.argmax(1)
+    for t in (1e-30, 1e-9, 1e-6):
+        opt = {"temperature": t, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
+        assert ops.sample_tokens(logits, u, **opt).tolist() == sample_by_definition(logits, u, **opt)
+        assert torch.equal(ops.sample_tokens(logits, u, temperature=t), best)
+    inf, nan = math.inf, math.nan
+    t = torch.tensor([inf, nan, -inf, 1e30, 1.0, 1.0], device=device)
+    p = torch.tensor([1.0, 1.0, 1.0, 0.5, nan, 1.0], device=device)
+    m = torch.tensor([0.0, 0.0, 0.0, 0.0, 0.0, nan], device=device)
+    logits[0, :1000] = -inf
+    got = ops.sample_tokens(logits, u, temperature=t, top_p=p, min_p=m).tolist()
+    even = 1000 + int(math.floor(float(u[0].double()) * 2001))       # 2001 weights of 1
+    assert got[0] == even and got[1] == int(logits[1].argmax()) and got[2] == int(logits[2].argmax())
+    plain = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
+    assert got[4:] == sample_by_definition(logits, u, **plain)[4:]
+    half = torch.sort(logits[3].double(), descending=True, stable=True).indices[:1501]
+    index = torch.sort(half).values                                   # 1501 >= 0.5 * 3001
+    assert got[3] == int(index[int(math.floor(float(u[3].double()) * 1501))])
+    first = ops.sample_tokens(logits, torch.full_like(u, nan), **plain)
+    assert torch.equal(first, ops.sample_tokens(logits, torch.zeros_like(u), **plain))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("vocab", [8, 9, 65543, 131071, 1 << 19])
+def test_sample_tokens_vocabularies(device, vocab):
+    """The smallest and largest rows, and cuts that keep a few, some thousand
+    and most of a row."""
+    logits = randn(2, vocab, seed=vocab % 1000, device=device).mul_(2.5).to(BF16)
+    for i, o in enumerate([dict(), dict(top_k=3), dict(top_k=300), dict(top_k=600), dict(top_k=3000, top_p=0.7),
+                           dict(top_k=7000, top_p=0.99), dict(top_p=0.3), dict(top_p=0.9999), dict(min_p=1e-5),
+                           dict(temperature=50.0, top_p=0.95)]):
+        opt = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, **o}
+        u = uniform(2, 110 + i, device)
+        assert ops.sample_tokens(logits, u, **opt).tolist() == sample_by_definition(logits, u, **opt), opt
 
 
 @pytest.mark.parametrize("device", DEVICES)
