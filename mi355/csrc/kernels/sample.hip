@@ -225,10 +225,11 @@ DEVINL int last_lane(int x) { return __builtin_amdgcn_readlane(x, 63); }
 template <typename I> DEVINL I wave_sum(I x) { return last_lane(wave_scan(x)); }
 
 struct Shared {
-  u64 hist[BINS];                        // and the logits of the last segment
+  u64 hist[BINS];
   u64 cand_k[CAP], cand_w[CAP], sum[CAP];
-  u64 list_k[LIST], list_w[LIST];
-  u64 seg[SEGS];
+  u64 list_k[LIST];
+  union { u64 list_w[LIST]; int list_i[LIST]; };
+  u64 seg[SEGS], last[SEG];
   u64 wave_tot[WAVES];
   u64 table[TABLE];
   float red[2][WAVES];
@@ -321,9 +322,9 @@ DEVINL void candidate(Shared& s, u64 key, u64 w) {
   if (to < CAP) { s.cand_k[to] = key; s.cand_w[to] = w; }
 }
 
-// All elements of at least `low` to the list, as far as it goes.  Where a
-// wave's logit goes follows from masks in scalar registers: a logit that no
-// lane lists costs a comparison.
+// All elements of at least `low` to the list, as far as it goes: their indices
+// first - where a wave's logit goes follows from masks in scalar registers, and
+// one that no lane lists costs a comparison - then, a lane each, their keys.
 template <typename T> DEVINL void list_from(Shared& s, const Row<T>& row, float low) {
   const int lane = threadIdx.x & 63;
   low = fmaxf(low, -3.402823466e38f);
@@ -344,10 +345,13 @@ template <typename T> DEVINL void list_from(Shared& s, const Row<T>& row, float 
       if (!who[e]) continue;
       const int at = to + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(who[e] >> 32),
                                                          __builtin_amdgcn_mbcnt_lo((unsigned)who[e], 0));
-      if (x[e] >= low && at < LIST) s.list_k[at] = rank_key(x[e], row.first(q) + e);
+      if (x[e] >= low && at < LIST) s.list_i[at] = row.first(q) + e;
       to += __popcll(who[e]);
     }
   });
+  __syncthreads();
+  const int n = min(s.list_n, LIST);
+  for (int i = threadIdx.x; i < n; i += THREADS) s.list_k[i] = rank_key(row.at(s.list_i[i]), s.list_i[i]);
   __syncthreads();
 }
 
@@ -368,6 +372,8 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   });
   if (t < TABLE) s.table[t] = EXP2_TABLE[t];
   for (int i = t; i < BINS; i += THREADS) s.hist[i] = 0;
+  s.seg[t] = 0;                                     // SEGS of them
+  if (t < SEG) s.last[t] = 0;
   if (t == 0) { s.cand_n = s.list_n = 0; s.found_bin = -1; s.greedy = 0x7fffffff; }
   float mx = wave_reduce_max(mine);
   float mn = -wave_reduce_max(mine > -INFINITY ? -mine : -INFINITY);
@@ -563,7 +569,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
       const double enough = p * (double)total;
       return [enough](u64 sum) { return sum > 0 && (double)sum >= enough; };
     };
-    clear(s);
+    if (border) clear(s);                           // else nothing was counted yet
     if (listed) {
       const int n = s.list_n;
       for (int i = t; i < n; i += THREADS) {
@@ -666,14 +672,10 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   // Kept weights in index order: a sum for each segment of 512, the segment
   // that the number falls into, and the logit in it.
   const int nseg = (V + SEG - 1) / SEG;
-  __syncthreads();
-  for (int i = t; i < nseg; i += THREADS) s.seg[i] = 0;
-  for (int i = t; i < SEG; i += THREADS) s.hist[i] = 0;
   auto kept = [&](float x, int idx) -> u64 {
     const u64 v = x > -INFINITY && rank_key(x, idx) >= border ? weight.of(x) : 0;
     return v >= min_w ? v : 0;
   };
-  __syncthreads();
   const int n_list = s.list_n;
   if (listed) {
     for (int i = t; i < n_list; i += THREADS) {
@@ -712,16 +714,16 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   if (listed) {
     for (int i = t; i < n_list; i += THREADS) {
       const int at = index_of(s.list_k[i]);
-      if (at / SEG == seg) s.hist[at % SEG] = s.list_w[i];
+      if (at / SEG == seg) s.last[at % SEG] = s.list_w[i];
     }
   } else if (t < SEG && seg * SEG + t < V) {
-    s.hist[t] = kept(row.at(seg * SEG + t), seg * SEG + t);
+    s.last[t] = kept(row.at(seg * SEG + t), seg * SEG + t);
   }
   __syncthreads();
   if (wave == 0) {
     u64 w[8], sum = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { w[e] = s.hist[lane * 8 + e]; sum += w[e]; }
+    for (int e = 0; e < 8; ++e) { w[e] = s.last[lane * 8 + e]; sum += w[e]; }
     const u64 want = s.last_want, end = wave_scan(sum);
     if (end - sum <= want && end > want) {
       u64 c = end - sum;
