@@ -172,16 +172,17 @@ template <typename T> struct Row {
       f(take8(r, q), q);
     }
   }
-  DEVINL unsigned bits_from(f32x8 x, float low) const {
+  DEVINL unsigned bits_from(f32x8 x, float low, float high) const {
     unsigned bits = 0;
+    low = fmaxf(low, -3.402823466e38f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bits |= x[e] >= low && x[e] > -INFINITY ? 1u << e : 0u;
+    for (int e = 0; e < 8; ++e) bits |= x[e] >= low && x[e] <= high ? 1u << e : 0u;
     return bits;
   }
-  // f(x, index) for the few elements that are at least `low`
-  template <typename F> DEVINL void each_from(float low, F f) const {
+  // f(x, index) for the few elements from `low` to `high`
+  template <typename F> DEVINL void each_from(float low, float high, F f) const {
     each1([&](f32x8 x, int q) {
-      unsigned bits = bits_from(x, low);
+      unsigned bits = bits_from(x, low, high);
 #pragma unroll 1
       while (bits) {
         const int b = __builtin_ctz(bits);
@@ -399,7 +400,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
     mx = mn = 0.f;
   }
   if (!(temp > 0.0) || k == 1 || p <= 0.0) {        // the first of the order
-    row.each_from(mx, [&](float, int idx) { atomicMin(&s.greedy, idx); });
+    row.each_from(mx, mx, [&](float, int idx) { atomicMin(&s.greedy, idx); });
     __syncthreads();
     if (t == 0) out[r] = s.greedy;
     return;
@@ -424,6 +425,10 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   auto low_of = [&](int b) {
     return b >= BINS - 2 || !(bin_scale > 0.f) ? -INFINITY : mx - (float)(b + 2) / bin_scale;
   };
+  // and one that is not below any of bins b..
+  auto high_of = [&](int b) {
+    return b < 2 || !(bin_scale > 0.f) ? INFINITY : mx - (float)(b - 1) / bin_scale;
+  };
 
   u64 border = 0;                                   // the last element kept; 0: all are
   bool ordered = false;                             // and top-p is done
@@ -445,7 +450,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
         if (bin_of(x) == bin && key >= floor_key) candidate(s, key, value(x));
       }
     } else {
-      row.each_from(low_of(bin), [&](float x, int idx) {
+      row.each_from(low_of(bin), high_of(bin), [&](float x, int idx) {
         const u64 key = rank_key(x, idx);
         if (bin_of(x) == bin && key >= floor_key) candidate(s, key, value(x));
       });
@@ -464,7 +469,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
       const int up = shift, bits = min(11, shift);
       shift -= bits;
       clear(s);
-      row.each_from(low_of(bin), [&](float x, int idx) {
+      row.each_from(low_of(bin), high_of(bin), [&](float x, int idx) {
         const u64 key = rank_key(x, idx);
         if (bin_of(x) != bin || key < floor_key || (up < 64 && (key >> up) != prefix)) return;
         // bin 0 holds the largest
@@ -604,6 +609,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
       // Only what is at least every thread's largest goes to the histogram at
       // first: the border is hardly ever below, and the atomics cost as much
       // as the weights.
+      float from = mn;
       u64 total = 0;
       auto weigh = [&](auto floored) {
         row.each1([&](f32x8 x, int q) {
@@ -612,32 +618,26 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
             u64 w = weight.of(x[e]);
             if (floored && rank_key(x[e], row.first(q) + e) < floor_key) w = 0;
             total += w;
-            if (x[e] >= mn) atomicAdd(&s.hist[bin_of(x[e])], w);
+            if (x[e] >= from) atomicAdd(&s.hist[bin_of(x[e])], w);
           }
         });
       };
-      if (floor_key) weigh(std::true_type());
-      else weigh(std::false_type());
-      total = wave_sum(total);
-      if (lane == 0) s.cand_w[wave] = total;
-      __syncthreads();
-      total = 0;
+#pragma unroll 1
+      for (int turn = 0; turn < 2; ++turn) {
+        total = 0;
+        if (floor_key) weigh(std::true_type());
+        else weigh(std::false_type());
+        total = wave_sum(total);
+        if (lane == 0) s.cand_w[wave] = total;
+        __syncthreads();
+        total = 0;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) total += s.cand_w[w];
-      find_bin(s, 0, total, need);
-      if (s.found_bin < 0) {
+        for (int w = 0; w < WAVES; ++w) total += s.cand_w[w];
+        find_bin(s, 0, total, need);
+        if (s.found_bin >= 0) break;
         clear(s);
         bin_scale = narrow / 3;
-        row.each1([&](f32x8 x, int q) {
-#pragma unroll 1
-          for (int e = 0; e < 8; ++e) {
-            const float v = Row<T>::pick(x, e);
-            if (v > -INFINITY && (!floor_key || rank_key(v, row.first(q) + e) >= floor_key))
-              atomicAdd(&s.hist[bin_of(v)], weight.of(v));
-          }
-        });
-        __syncthreads();
-        find_bin(s, 0, total, need);
+        from = -3.402823466e38f;
       }
       cut_in_bin(s.found_bin, s.found_before, floor_key,
                  [&](float x) { return weight.of(x); }, need(total));
