@@ -264,11 +264,14 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 // Tiles of 128 x 128 once there are 128 of them for the 256 CUs, else of
 // 64 x 64 once there are 128, else of 32 x 32: 256 rows by 10240 x 2048 take
 // 27, 33 and 52 us, by 4096 x 768 13, 6.4 and 9.2 us, by 768 x 2048 25, 12 and
-// 7.6 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).
+// 7.6 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Where there are
+// few tiles and a long K, tiles of 64 x 64 share K, in runs of 512 and more,
+// and a second kernel adds their fp32 sums: 64 rows by 4096 x 10240 34 -> 20 us,
+// 128 by 2048 x 5120 18 -> 14; 64 by 1024 x 2816, too short, 9.0 and 8.9.
 // ---------------------------------------------------------------------------
 template <typename T, int MT, int NT, int WN>
 __global__ void __launch_bounds__(128 * WN)
-w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
+w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ part, int run, Args a) {
   using vec = typename Frag<T>::vec;
   constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * NT * WN, KC = 128, LD = KC + 8;
   constexpr int LOADS = BM * KC / 8 / THREADS;       // 16-byte pieces of x a thread brings
@@ -276,6 +279,7 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
   const int wm = wave & 1, wn = wave >> 1;
+  const int k_at = blockIdx.z * run, k_end = min(k_at + run, a.K);   // this workgroup's part of K
   const int m_at = blockIdx.x * BM, n0 = blockIdx.y * BN + wn * 16 * NT + c16;
   int row_e[NT];
   const unsigned char *crow[NT], *erow[NT];
@@ -311,7 +315,7 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     }
   };
   auto stage = [&](const Piece& p, int k0, int buf) {
-    const unsigned keep = k0 + xk < a.K ? 0xffffffffu : 0u;
+    const unsigned keep = k0 + xk < k_end ? 0xffffffffu : 0u;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
       *reinterpret_cast<u32x4*>(&lds[buf][(threadIdx.x + THREADS * i) / (KC / 8) * LD + xk]) = p.x[i] & keep;
@@ -332,7 +336,7 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   // multiplies the piece in `buf`, whose weights are in `now`, while that after
   // the next is loaded
   auto step = [&](int k0, Piece& now, const Piece& next, int buf) {
-    const unsigned keep = k0 + 32 * g < a.K ? 0xffffffffu : 0u;
+    const unsigned keep = k0 + 32 * g < k_end ? 0xffffffffu : 0u;
     u32x4 w[NT];
     float scale[NT];
 #pragma unroll
@@ -354,12 +358,12 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     stage(next, k0 + KC, buf ^ 1);
     lds_barrier();
   };
-  load(ahead[0], 0);
-  load(ahead[1], KC);
-  stage(ahead[0], 0, 0);
+  load(ahead[0], k_at);
+  load(ahead[1], k_at + KC);
+  stage(ahead[0], k_at, 0);
   lds_barrier();
   // in pairs; of an odd number of pieces the last is multiplied by zeros
-  for (int k0 = 0; k0 < a.K; k0 += 2 * KC) {
+  for (int k0 = k_at; k0 < k_end; k0 += 2 * KC) {
     step(k0, ahead[0], ahead[1], 0);
     step(k0 + KC, ahead[1], ahead[0], 1);
   }
@@ -373,9 +377,23 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int m = m_at + wm * 16 * MT + 16 * t + 4 * g + r;
-        if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(acc[t][u][r] * back);
+        if (m >= a.M) continue;
+        if (part) part[((long)blockIdx.z * a.M + m) * a.N + n] = acc[t][u][r];
+        else y[(long)m * a.N + n] = DT<T>::from_f32(acc[t][u][r] * back);
       }
   }
+}
+
+// The sum over parts of K, in their order, and the rows' scales.
+template <typename T>
+__global__ void __launch_bounds__(256)
+w4_add_parts(const float* __restrict__ part, T* __restrict__ y, int parts, Args a) {
+  const long mn = (long)a.M * a.N, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= mn) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) s += part[p * mn + i];
+  y[i] = DT<T>::from_f32(s * row_scale(a.row_exp[i % a.N]));
 }
 
 }  // namespace
@@ -416,11 +434,23 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
                row_exp.data_ptr<unsigned char>(), (int)M, (int)N, (int)K, (long)x.stride(0)};
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    auto launch = [&](auto kernel, dim3 grid, int threads, long lds) {
-      hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, stream, (const T*)x.data_ptr(),
-                         (T*)y.data_ptr(), a);
-    };
     const auto up = [](long n, long by) { return (n + by - 1) / by; };
+    auto launch = [&](auto kernel, dim3 grid, int threads, long lds, auto... more) {
+      hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, stream, (const T*)x.data_ptr(),
+                         (T*)y.data_ptr(), more..., a);
+    };
+    auto many = [&](auto kernel, dim3 grid, int threads, long parts) {
+      const long run = up(up(K, parts), 128) * 128;
+      parts = up(K, run);
+      grid.z = parts;
+      torch::Tensor part;
+      if (parts > 1) part = at::empty({parts * M * N}, x.options().dtype(torch::kFloat));
+      float* p = parts > 1 ? part.data_ptr<float>() : nullptr;
+      launch(kernel, grid, threads, 0, p, (int)run);
+      if (parts > 1)
+        hipLaunchKernelGGL(w4_add_parts<T>, dim3(up(M * N, 256)), dim3(256), 0, stream, p,
+                           (T*)y.data_ptr(), (int)parts, a);
+    };
     const auto tiles = [&](long t) { return dim3(up(M, t), up(N, t)); };
     const auto count = [](dim3 d) { return (long)d.x * d.y; };
     const long copy = M * (K + 8) * 2;              // x in LDS
@@ -432,11 +462,13 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
       else if (M <= 8) launch(w4_few_rows<T, 2, 8>, dim3(up(N, 32)), 512, 0);
       else launch(w4_few_rows<T, 4, 8>, dim3(up(N, 64)), 512, 0);
     } else if (count(tiles(128)) >= 128) {
-      launch(w4_many_rows<T, 4, 2, 4>, tiles(128), 512, 0);
+      many(w4_many_rows<T, 4, 2, 4>, tiles(128), 512, 1);
+    } else if (K >= 4096 && count(tiles(64)) < 256) {
+      many(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, std::min(up(256, count(tiles(64))), K / 512));
     } else if (count(tiles(64)) >= 128) {
-      launch(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, 0);
+      many(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, 1);
     } else {
-      launch(w4_many_rows<T, 1, 1, 2>, tiles(32), 256, 0);
+      many(w4_many_rows<T, 1, 1, 2>, tiles(32), 256, 1);
     }
   };
   if (x.scalar_type() == torch::kBFloat16) go(__hip_bfloat16());

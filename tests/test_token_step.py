@@ -67,7 +67,9 @@ def check_linear(x, w, y):
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 16, 64), (1, 2304, 768), (3, 17, 96), (5, 48, 2048),
                                    (16, 100, 1024), (17, 33, 160), (31, 129, 128), (64, 65, 512),
-                                   (65, 200, 736), (130, 257, 320), (256, 64, 4096), (300, 512, 768)])
+                                   (65, 200, 736), (130, 257, 320), (256, 64, 4096), (300, 512, 768),
+                                   (40, 130, 4128), (100, 2050, 4640), (260, 8200, 96), (9, 8200, 160), (8, 8200, 4640), (129, 2700, 128),
+                                   (2, 16390, 288)])
 def test_linear_w4(device, dtype, m, n, k):
     w = random_w4(n, k, seed=m * 7 + n, device=device)
     x = randn(m, k, seed=k, device=device, dtype=dtype)
