@@ -23,9 +23,10 @@
 // One workgroup a row; the row is read from memory once, and a few times from
 // the L2 after that.  What bounds it is one CU's instruction rate (an
 // instruction for every logit of a 32128 row is 0.2 us; a weight is about 20 of
-// them) and, in code that runs once, instruction fetch: passes over the row are
-// short loops, and what happens to few elements is left to a compact inner loop
-// over a bit mask.
+// them, 7 us a row) and, for a small top-k, the latency of its dozen steps.
+// One row of 32128 with top-k 50 and top-p 10 us; 256 rows, nucleus sampling,
+// 27 us (reading them: 3.3 us); 33 rows of 50257 in fp32, top-k 100 to 300,
+// 17 us; 52647 logits with a nucleus of some 10000, the longest path, 62 us.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
