@@ -258,13 +258,15 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup of 2 x WN waves makes 32*MT rows by 16*NT*WN outputs.
 // x goes through LDS, 128 of K at a time in two buffers (two pieces are on
-// their way in registers while one is multiplied; rows lie 16 bytes apart from
-// a multiple of 256, so that 16 rows at one k are in different banks); weights
-// go from memory to registers as above, converted once for MT tiles of rows.
+// their way in registers while one is multiplied); weights go from memory to
+// registers as above, converted once for MT tiles of rows.  LDS holds the 32 k
+// of a lane group as a plane of its own, rows 80 bytes apart and planes a
+// multiple of 256: sixteen rows at one k are in different banks, in whichever
+// lane groups the hardware takes them.
 // Tiles of 128 x 128 once there are 128 of them for the 256 CUs, else of
 // 64 x 64 once there are 128, else of 32 x 32: 256 rows by 10240 x 2048 take
-// 27, 33 and 52 us, by 4096 x 768 13, 6.4 and 9.2 us, by 768 x 2048 25, 12 and
-// 7.6 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Where there are
+// 25, 34 and 53 us, by 4096 x 768 11, 6.6 and 9.5 us, by 768 x 2048 23, 12 and
+// 7.8 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Where there are
 // few tiles and a long K, tiles of 64 x 64 share K, in runs of 512 and more,
 // and a second kernel adds their fp32 sums: 64 rows by 4096 x 10240 34 -> 20 us,
 // 128 by 2048 x 5120 18 -> 14; 64 by 1024 x 2816, too short, 9.0 and 8.9.
@@ -273,9 +275,10 @@ template <typename T, int MT, int NT, int WN>
 __global__ void __launch_bounds__(128 * WN)
 w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ part, int run, Args a) {
   using vec = typename Frag<T>::vec;
-  constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * NT * WN, KC = 128, LD = KC + 8;
+  constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * NT * WN, KC = 128;
+  constexpr int LD = 40, PLANE = BM * LD;         // elements: a row of 32 k, 32 k of all rows
   constexpr int LOADS = BM * KC / 8 / THREADS;       // 16-byte pieces of x a thread brings
-  __shared__ alignas(16) T lds[2][BM * LD];
+  __shared__ alignas(256) T lds[2][4 * PLANE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
   const int wm = wave & 1, wn = wave >> 1;
@@ -297,16 +300,15 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
     u32x4 x[LOADS], w[NT];
     int e[NT];
   } ahead[2];
-  const T* xrow[LOADS];
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i)
-    xrow[i] = x + min(m_at + (int)(threadIdx.x + THREADS * i) / (KC / 8), a.M - 1) * a.ldx;
-  const int xk = threadIdx.x % (KC / 8) * 8;        // the same k for all of a thread's pieces
-  static_assert(THREADS % (KC / 8) == 0, "");
+  // piece p of x: 8 of k at 8 * (p % 4) of row p / 4 % BM of plane p / (4 * BM)
+  const int xrow = threadIdx.x / 4 % BM, xk = threadIdx.x % 4 * 8;
+  const T* xat = x + min(m_at + xrow, a.M - 1) * a.ldx;
+  static_assert(THREADS % (4 * BM) == 0, "the same row for all of a thread's pieces");
+  auto plane = [&](int i) { return (int)(threadIdx.x + THREADS * i) / (4 * BM); };
   auto load = [&](Piece& p, int k0) {
-    const int k = min(k0 + xk, a.K - 8);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) p.x[i] = *reinterpret_cast<const u32x4*>(xrow[i] + k);
+    for (int i = 0; i < LOADS; ++i)
+      p.x[i] = *reinterpret_cast<const u32x4*>(xat + min(k0 + 32 * plane(i) + xk, a.K - 8));
     const int kk = min(k0 + 32 * g, a.K - 32);      // K is a multiple of 32
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -315,10 +317,11 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
     }
   };
   auto stage = [&](const Piece& p, int k0, int buf) {
-    const unsigned keep = k0 + xk < k_end ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      *reinterpret_cast<u32x4*>(&lds[buf][(threadIdx.x + THREADS * i) / (KC / 8) * LD + xk]) = p.x[i] & keep;
+    for (int i = 0; i < LOADS; ++i) {
+      const unsigned keep = k0 + 32 * plane(i) < k_end ? 0xffffffffu : 0u;
+      *reinterpret_cast<u32x4*>(&lds[buf][plane(i) * PLANE + xrow * LD + xk]) = p.x[i] & keep;
+    }
   };
   // orders LDS alone: a plain barrier would wait for the loads on their way
   auto lds_barrier = [] {
@@ -342,7 +345,7 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
 #pragma unroll
     for (int u = 0; u < NT; ++u) { w[u] = now.w[u] & keep; scale[u] = group_scale(now.e[u], row_e[u]); }
     load(now, k0 + 2 * KC);
-    const T* row = &lds[buf][(wm * 16 * MT + c16) * LD + 32 * g];
+    const T* row = &lds[buf][g * PLANE + (wm * 16 * MT + c16) * LD];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       vec xf[MT];
