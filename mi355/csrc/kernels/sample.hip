@@ -407,7 +407,9 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
     return;
   }
 
-  const double slope = 46.16624130844683 / temp;
+  // finite, so that the maximum's distance of 0 stays 0: under 1e-300 nothing but
+  // the maximum weighs anything either way
+  const double slope = 46.16624130844683 / fmax(temp, 1e-300);
   const Weights weight{(double)mx, slope, s.table};
   floor_p = floor_p > 1.0 ? 1.0 : floor_p;          // the maximum always stays
   const u64 min_w = floor_p > 0.0 ? (u64)__builtin_rint(floor_p * ONE) : 0;
@@ -434,6 +436,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
   u64 border = 0;                                   // the last element kept; 0: all are
   bool ordered = false;                             // and top-p is done
   bool listed = false;                              // the list holds all up to the border
+  bool counted = false;                             // the histogram was used
 
   // Leaves border, and the list where what is not behind `bin` fits (all that
   // the cut keeps, and a few more).  Of `bin`, what is not below floor_key and
@@ -551,22 +554,23 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
         listed = done = ordered = true;
       }
       if (!done) {
-      clear(s);
-      if (t == 0) s.list_n = 0;
+        clear(s);
+        if (t == 0) s.list_n = 0;
       }
     }
     if (!done) {
-    bin_scale = narrow / 3;
-    row.each4([&](f32x8 x, int) {
+      counted = true;
+      bin_scale = narrow / 3;
+      row.each4([&](f32x8 x, int) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (x[e] > -INFINITY) atomicAdd(&s.hist[bin_of(x[e])], (u64)1);
-    });
-    __syncthreads();
-    find_bin(s, 0, 0, [&](u64) { return reached; });
-    // fewer than k may be there: then all stay
-    if (s.found_bin >= 0)
-      cut_in_bin(s.found_bin, s.found_before, 0, [](float) { return (u64)1; }, reached);
+        for (int e = 0; e < 8; ++e)
+          if (x[e] > -INFINITY) atomicAdd(&s.hist[bin_of(x[e])], (u64)1);
+      });
+      __syncthreads();
+      find_bin(s, 0, 0, [&](u64) { return reached; });
+      // fewer than k may be there: then all stay
+      if (s.found_bin >= 0)
+        cut_in_bin(s.found_bin, s.found_before, 0, [](float) { return (u64)1; }, reached);
     }
   }
 
@@ -575,7 +579,7 @@ sample_kernel(const T* __restrict__ logits, long ld, int V, const void* __restri
       const double enough = p * (double)total;
       return [enough](u64 sum) { return sum > 0 && (double)sum >= enough; };
     };
-    if (border) clear(s);                           // else nothing was counted yet
+    if (counted) clear(s);                          // also where fewer than k were there
     if (listed) {
       const int n = s.list_n;
       for (int i = t; i < n; i += THREADS) {
@@ -788,7 +792,7 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
   if (logits.scalar_type() == torch::kBFloat16) SAMPLE(__hip_bfloat16);
   else if (logits.scalar_type() == torch::kHalf) SAMPLE(__half);
   else if (logits.scalar_type() == torch::kFloat) SAMPLE(float);
-  else TORCH_CHECK(false, "sample_tokens: bf16, fp16 or fp32 logits, got ", logits.scalar_type());
+  else VALUE_CHECK(false, "sample_tokens takes bf16, fp16 or fp32 logits on a GPU, got ", logits.scalar_type());
 #undef SAMPLE
   HIP_CHECK_KERNEL();
   return out;

@@ -596,6 +596,42 @@ def test_sample_tokens_odd_options(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("temperature", [1e-300, 1e-310, 5e-324])
+def test_sample_tokens_tiniest_temperatures(device, dtype, temperature):
+    """Down to the smallest number over 0 the maximum has weight 1 and equal
+    ones share: nothing else weighs anything."""
+    logits = randn(5, 900, seed=103, device=device, dtype=dtype)
+    logits[2, [5, 70, 800]] = logits[2].max() + 1
+    for opt in (dict(), dict(top_k=20), dict(top_k=100, top_p=0.9), dict(top_p=0.9)):
+        opt = {"temperature": temperature, "top_k": 0, "top_p": 1.0, "min_p": 0.0} | opt
+        for r in (0.0, 0.5, 0.9999):
+            got = ops.sample_tokens(logits, torch.full((5,), r, device=device), **opt)
+            want = logits.double().argmax(1)
+            want[2] = 70 if r == 0.5 else 800 if r > 0.5 else 5
+            assert got.tolist() == want.tolist(), (opt, r)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_tokens_fewer_than_top_k(device):
+    """A top-k that finds fewer than it may keep leaves nothing behind for the
+    nucleus: fifty weights of 1 and one of 2^-24, of which 25 * 2^-44 have to
+    be in."""
+    v, small = 4000, -16.635532333438686
+    logits = torch.full((8, v), -math.inf, device=device)
+    at = torch.arange(50, device=device) * 61 + 3
+    logits[:, at] = 0.0
+    logits[:, 3900] = small
+    e = math.exp(float(torch.tensor(small)))
+    p = (50 + 25 * 2.0 ** -44) / (50 + e)
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.99, 1 - 2.0 ** -40, 1 - 2.0 ** -41, 1.0], dtype=torch.float64, device=device)
+    opt = {"temperature": 1.0, "top_k": 600, "top_p": p, "min_p": 0.0}
+    got = ops.sample_tokens(logits, u, **opt).tolist()
+    assert got == sample_by_definition(logits, u, **opt)
+    assert got[5:] == [3900] * 3
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("vocab", [8, 9, 65543, 131071, 1 << 19])
 def test_sample_tokens_vocabularies(device, vocab):
     """The smallest and largest rows, and cuts that keep a few, some thousand
