@@ -175,6 +175,10 @@ w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   add_waves<T, NT, WAVES>(part, acc, n0, y, a);
 }
 
+// Elements of a row of x in LDS: zeros behind K as far as a wave's pieces reach
+// (a repeated infinity would meet a weight of 0), and 16 bytes between rows.
+__host__ __device__ constexpr int lds_row(int K) { return (K + 255) / 256 * 256 + 8; }
+
 // The same with x in LDS, for few enough rows that a workgroup's copy is small
 // beside its weights: of the 64 lanes that the matrix instruction has for x only
 // M in 16 hold a row (the others repeat the last; their sums are not stored),
@@ -192,7 +196,8 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c16 = lane & 15;
   const int n0 = blockIdx.x * (16 * NT) + c16;
-  const int LD = a.K + 8;
+  static_assert(U <= 2, "lds_row()");
+  const int LD = lds_row(a.K);
   int row_e[NT];
   const unsigned char *crow[NT], *erow[NT];
 #pragma unroll
@@ -225,9 +230,11 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   };
   constexpr int RUN = WAVES * 128 * U;
   Piece next = load(wave * 128 * U);
-  for (int i = threadIdx.x * 8; i < a.M * a.K; i += WAVES * 64 * 8) {
-    const int m = i / a.K, k = i - m * a.K;
-    *reinterpret_cast<u32x4*>(xs + m * LD + k) = *reinterpret_cast<const u32x4*>(x + m * a.ldx + k);
+  for (int i = threadIdx.x * 8; i < a.M * LD; i += WAVES * 64 * 8) {
+    const int m = i / LD, k = i - m * LD;
+    u32x4 v = u32x4{0u, 0u, 0u, 0u};
+    if (k < a.K) v = *reinterpret_cast<const u32x4*>(x + m * a.ldx + k);
+    *reinterpret_cast<u32x4*>(xs + i) = v;
   }
   __syncthreads();
   f32x4 acc[NT];
@@ -239,7 +246,7 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     if (k0 + RUN < a.K) next = load(k0 + RUN);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int k = min(k0 + 128 * j + 32 * g, a.K - 32);
+      const int k = k0 + 128 * j + 32 * g;
       float scale[NT];
 #pragma unroll
       for (int u = 0; u < NT; ++u) scale[u] = group_scale(p.e[j][u], row_e[u]);
@@ -456,7 +463,7 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
     };
     const auto tiles = [&](long t) { return dim3(up(M, t), up(N, t)); };
     const auto count = [](dim3 d) { return (long)d.x * d.y; };
-    const long copy = M * (K + 8) * 2;              // x in LDS
+    const long copy = M * lds_row(K) * 2;           // x in LDS
     if (M <= 8 && copy <= 56 * 1024) {
       if (M <= 2 && N >= 16384) launch(w4_lds_rows<T, 1, 2, 4>, dim3(up(N, 16)), 256, copy);
       else launch(w4_lds_rows<T, 1, 1, 8>, dim3(up(N, 16)), 512, copy);

@@ -106,6 +106,30 @@ def test_linear_w4_far_exponents(device, dtype):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 32), (2, 24, 96), (1, 16400, 288), (8, 40, 416), (12, 40, 160),
+                                   (12, 8210, 160), (40, 40, 416), (70, 70, 4128), (130, 8200, 160)])
+def test_linear_w4_infinite_inputs(device, dtype, m, n, k):
+    """An infinity makes infinite outputs (no NaN) of its own row alone, also
+    among the last inputs; NaN makes NaN."""
+    codes = torch.full((n, k // 2), 0x22, dtype=torch.uint8, device=device)      # ones
+    w = ops.W4Weight(codes, torch.full((n, k // 32), 127, dtype=torch.uint8, device=device))
+    x = torch.ones(m, k, device=device, dtype=dtype)
+    x[m - 1, k - 1] = math.inf
+    if m > 1:
+        x[0, k - 32] = -math.inf
+    if m > 2:
+        x[1, k - 7] = math.nan
+    y = ops.linear_w4(x, w)
+    assert bool((y[m - 1] == math.inf).all())
+    if m > 1:
+        assert bool((y[0] == -math.inf).all())
+    if m > 2:
+        assert bool(y[1].isnan().all()) and bool((y[2:m - 1] == k).all() or dtype == BF16)
+        assert bool(y[2:m - 1].isfinite().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_linear_w4_same_twice(device):
     w = random_w4(500, 1024, seed=8, device=device)
     x = randn(20, 1024, seed=9, device=device, dtype=BF16)
