@@ -792,7 +792,7 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
   if (logits.scalar_type() == torch::kBFloat16) SAMPLE(__hip_bfloat16);
   else if (logits.scalar_type() == torch::kHalf) SAMPLE(__half);
   else if (logits.scalar_type() == torch::kFloat) SAMPLE(float);
-  else VALUE_CHECK(false, "sample_tokens takes bf16, fp16 or fp32 logits on a GPU, got ", logits.scalar_type());
+  else TORCH_CHECK(false, "sample_tokens takes bf16, fp16 or fp32 logits on a GPU, got ", logits.scalar_type());
 #undef SAMPLE
   HIP_CHECK_KERNEL();
   return out;
