@@ -340,16 +340,6 @@ DEVINL bf16x8 v_frag(unsigned c0, unsigned c1, float scale) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// the first n of 16 bytes
-DEVINL u32x4 keep_bytes(u32x4 x, int n) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = min(max(n - 4 * i, 0), 4);
-    x[i] &= k == 4 ? 0xffffffffu : (1u << (8 * k)) - 1u;
-  }
-  return x;
-}
-
 struct AttnArgs {
   const float* bias;   // (1 or B, Hq, width) or null
   const float* kpad;   // (B, width) or null
