@@ -336,7 +336,7 @@ class T5DenseGatedActDense(nn.Module):
         # fused on its output (no gate/up split views, no grad cat)
         p = self.dropout.p if self.training else 0.0
         h = ops.geglu_packed(ops.linear(x, self.wi.weight), p_drop=p,
-                             salt=self.wi.weight.data_ptr() if p > 0 else 0)
+                             salt=self.wi.weight.data_ptr())
         return ops.linear(h, self.wo.weight)
 
 

@@ -74,6 +74,9 @@ class W4Weight(torch.nn.Module):
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return torch_ref.w4_dequantize(self.codes, self.exps).to(dtype)
 
+    def data_ptr(self) -> int:
+        return self.codes.data_ptr()
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear_w4(x, self)
 
@@ -85,15 +88,20 @@ class W4Weight(torch.nn.Module):
 def quantize_w4(weight: torch.Tensor) -> W4Weight:
     """The nearest :class:`W4Weight` of a finite (N, K) weight: for each group
     of 32 inputs that power of two, of the two next to amax/6, whose rounded
-    codes are off by the smaller sum of squares."""
+    codes are off by the smaller sum of squares.  Waits for the device once, to
+    refuse what is not finite."""
     if weight.dim() != 2 or weight.shape[1] % W4Weight.GROUP or not weight.shape[1]:
         raise ValueError(f"quantize_w4 takes (N, K) with K a multiple of 32, got {tuple(weight.shape)}")
+    if not torch.isfinite(weight).all():
+        raise ValueError("quantize_w4 takes a finite weight")
     return W4Weight(*torch_ref.w4_quantize(weight))
 
 
 def linear_w4(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     """``x @ w.T`` for x (..., K) in bf16 or fp16: sums in 32 bits, one rounding
-    at the end.  Any number of rows; made for the few that decoding has."""
+    at the end.  Any number of rows; made for the few that decoding has.  The
+    largest scale of a row of w is multiplied in after its sum: sums of x times
+    codes have to stay in fp32's range (inputs under 2^125 / K do)."""
     if x.is_cuda and _use_hip(x):
         b = w._buffers
         return _load_ext().w4_linear(x, b["codes"], b["exps"], b["row_exp"])
@@ -132,7 +140,9 @@ class KVCache8:
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "KVCache8":
-        """A cache on buffers that the caller holds (shared, not copied)."""
+        """A cache on buffers that the caller holds (shared, not copied).  The
+        scales have to be powers of two from 2^-120 to 2^120, as appends make
+        them; that is not checked."""
         b, h, nb, d, block = v.shape if v.dim() == 5 else (0,) * 5
         if block != cls.BLOCK or d not in (32, 64, 128) or k.shape != (b, h, nb * block, d) \
                 or k_scale.shape != (b, h, nb) or v_scale.shape != (b, h, nb):

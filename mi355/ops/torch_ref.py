@@ -141,14 +141,14 @@ def w4_dequantize(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
     """(N, K/2) codes and (N, K/32) exponents -> fp32 (N, K)."""
     n, half = codes.shape
     table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
-    nibbles = torch.stack([codes & 15, codes >> 4], -1).view(n, 2 * half)
+    nibbles = torch.stack([codes & 15, codes >> 4], -1).view(n, half // 16, 32)
     scale = torch.ldexp(torch.ones((), device=codes.device), exps.int() - 127)
-    return (table[nibbles.int()].view(n, -1, 32) * scale[..., None]).view(n, -1)
+    return (table[nibbles.int()] * scale[..., None]).view(n, 2 * half)
 
 
 def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     n, k = weight.shape
-    w = weight.float().view(n, -1, 32)
+    w = weight.float().contiguous().view(n, k // 32, 32)
     amax = w.abs().amax(-1, keepdim=True)
     # 6 * 2^e >= amax for the upper of the two powers of two
     _, e = torch.frexp(amax / 6)
@@ -171,7 +171,7 @@ def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
             take = err < best[0]
             best = (None, torch.where(take, code, best[1]), torch.where(take, ee, best[2]))
     code = best[1].view(n, k).to(torch.uint8)
-    return code[:, 0::2] | code[:, 1::2] << 4, (best[2].view(n, -1) + 127).to(torch.uint8)
+    return code[:, 0::2] | code[:, 1::2] << 4, (best[2].view(n, k // 32) + 127).to(torch.uint8)
 
 
 def linear_w4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:

@@ -159,3 +159,23 @@ def test_captured_loop_matches_eager(quantized, options):
         junk = [torch.randn(512, 512, device="cuda") for _ in range(8)]     # eager work that reuses freed memory
         del junk
     assert not getattr(m, "_gen_graph_warned", False) and m._gen_graph is not None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_w4_decoder_with_dropout(device):
+    """In training mode without gradients the 4-bit decoder drops out like any
+    other; with gradients it is refused."""
+    m = model(device)
+    m.quantize_decoder_w4()
+    for mod in m.modules():
+        if hasattr(mod, "dropout") and isinstance(mod.dropout, torch.nn.Dropout):
+            mod.dropout.p = 0.1
+    m.train()
+    ids, mask = prompt(device)
+    out = m.generate(input_ids=ids, attention_mask=mask, max_new_tokens=4, min_new_tokens=4)
+    assert out.shape == (3, 4)
+    with torch.no_grad():
+        loss = m(input_ids=ids, attention_mask=mask, labels=ids).loss
+    assert bool(loss.isfinite())
+    with pytest.raises(RuntimeError):
+        m(input_ids=ids, attention_mask=mask, labels=ids)

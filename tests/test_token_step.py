@@ -130,6 +130,20 @@ def test_linear_w4_infinite_inputs(device, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_w4_empty_strided_and_refused(device):
+    """A weight without rows, one that is a view, and what cannot be quantized."""
+    w = ops.quantize_w4(torch.zeros(0, 64, device=device))
+    assert w.shape == (0, 64) and w.dequantize().shape == (0, 64)
+    assert ops.linear_w4(torch.ones(3, 64, device=device, dtype=BF16), w).shape == (3, 0)
+    weight = randn(64, 40, seed=11, device=device)
+    assert torch.equal(ops.quantize_w4(weight.t()).codes, ops.quantize_w4(weight.t().contiguous()).codes)
+    for bad in (math.nan, math.inf, -math.inf):
+        weight[5, 7] = bad
+        with pytest.raises(ValueError):
+            ops.quantize_w4(weight.t())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_linear_w4_same_twice(device):
     w = random_w4(500, 1024, seed=8, device=device)
     x = randn(20, 1024, seed=9, device=device, dtype=BF16)
