@@ -71,9 +71,9 @@ __constant__ const u64 EXP2_TABLE[TABLE] = {
 };
 
 // A larger float has a larger key; with the index: one order over all elements
-// of a row, larger first, then the lower index.
+// of a row, larger first, then the lower index.  -0 becomes 0: they are equal.
 DEVINL u64 rank_key(float x, int idx) {
-  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const unsigned u = __builtin_bit_cast(unsigned, x + 0.f);
   return (u64)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (unsigned)~idx;
 }
 DEVINL float value_of(u64 key) {

@@ -651,6 +651,23 @@ def test_sample_tokens_tiniest_temperatures(device, dtype, temperature):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("vocab", [44, 4619, 32128])
+def test_sample_tokens_zeros_of_both_signs(device, dtype, vocab):
+    """0 and -0 are equal: the lower index comes first, at every kind of border."""
+    zeros = torch.where(torch.arange(vocab) % 3 == 0, -0.0, 0.0)
+    levels = (randn(4, vocab, seed=104, device="cpu") * 2).round() / 2
+    levels[0] = zeros
+    levels[1, 5:] = zeros[5:]
+    logits = levels.to(device=device, dtype=dtype)
+    u = torch.tensor([0.9, 0.71, 0.93, 0.4], device=device)
+    for opt in (dict(top_k=30), dict(top_k=vocab // 2), dict(top_k=vocab * 2 // 3), dict(top_p=0.517),
+                dict(top_p=0.7131, top_k=vocab * 3 // 4), dict(temperature=30.0, top_p=0.517)):
+        opt = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0} | opt
+        assert ops.sample_tokens(logits, u, **opt).tolist() == sample_by_definition(logits, u, **opt), opt
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_sample_tokens_fewer_than_top_k(device):
     """A top-k that finds fewer than it may keep leaves nothing behind for the
     nucleus: fifty weights of 1 and one of 2^-24, of which 25 * 2^-44 have to
