@@ -228,6 +228,8 @@ def kv8_append(kc, vc, k_scale, v_scale, k, v, start, counts=None) -> None:
 
 def decode_attention_kv8(q, k, v, k_scale, v_scale, lengths, bias, kpad, scale, max_len):
     b, h, cap, d = k.shape
+    if max_len == 0:
+        return torch.zeros_like(q)
     kf, vf = kv8_values(k, v, k_scale, v_scale)
     kf, vf = kf[:, :, :max_len], vf[:, :, :max_len]
     there = torch.arange(max_len, device=q.device) < (
@@ -243,8 +245,6 @@ def decode_attention_kv8(q, k, v, k_scale, v_scale, lengths, bias, kpad, scale, 
     if kpad is not None:
         s = s + kpad[:, None, None, :max_len].float()
     s = torch.where(there[:, None, None], s, -math.inf)
-    if max_len == 0:
-        return torch.zeros_like(q)
     m = s.amax(-1, keepdim=True)
     p = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
     l = p.sum(-1, keepdim=True)

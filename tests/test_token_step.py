@@ -464,6 +464,21 @@ def test_decode_attention_kv8_max_len(device):
         check_attention(q, cache, lengths, None, None, 1.0, out, max_len=min(max_len or 256, 256))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("capacity", [0, 70])
+def test_decode_attention_kv8_no_length_with_masks(device, capacity):
+    """No keys at all, however that is said, with masks of any width: 0."""
+    cache = ops.KVCache8(2, 3, capacity, 64, device=device)
+    q = randn(2, 6, 1, 64, seed=105, device=device, dtype=BF16)
+    none = torch.zeros(2, dtype=torch.int32, device=device)
+    for width in (0, 5):
+        bias, kpad = torch.zeros(1, 6, 1, width, device=device), torch.zeros(2, width, device=device)
+        for lengths, most in ((0, None), (none, 0), (none + 9, 0), (none, min(width, capacity))):
+            for masks in (dict(), dict(bias=bias), dict(kpad=kpad), dict(bias=bias, kpad=kpad)):
+                out = ops.decode_attention_kv8(q, cache, lengths, max_len=most, **masks)
+                assert out.shape == q.shape and not bool(out.any())
+
+
 @gpu
 def test_kv8_offsets_over_32_bits():
     """Heads whose codes begin 4.3 GB into the cache."""
