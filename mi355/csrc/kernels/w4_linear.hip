@@ -273,7 +273,9 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 // Tiles of 128 x 128 once there are 128 of them for the 256 CUs, else of
 // 64 x 64 once there are 128, else of 32 x 32: 256 rows by 10240 x 2048 take
 // 25, 34 and 53 us, by 4096 x 768 11, 6.6 and 9.5 us, by 768 x 2048 23, 12 and
-// 7.8 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Where there are
+// 7.8 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Four waves of 64 x
+// 64 read half as much LDS as eight of 64 x 32, but 30 us, one for each SIMD, is
+// more than 25.  Where there are
 // few tiles and a long K, tiles of 64 x 64 share K, in runs of 512 and more,
 // and a second kernel adds their fp32 sums: 64 rows by 4096 x 10240 34 -> 20 us,
 // 128 by 2048 x 5120 18 -> 14; 64 by 1024 x 2816, too short, 9.0 and 8.9.
