@@ -283,8 +283,9 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
 // and the columns of a head are summed at the end.  So a lane makes GP weights,
 // not 16, and a token's weight is made once.
 //
-// P is split into two bf16 numbers, p = hi + lo (16 significant bits, so P
-// adds no error beside the output's own rounding).  The reference m that is
+// P is split into three bf16 numbers, p = hi + mid + lo, 8 significant bits
+// each: all of its 24.  (With two a weight is off by up to 2^-18, and ten times
+// as many outputs land a step beside the nearest one.)  The reference m that is
 // subtracted in the exponent is raised, and what was summed rescaled, only when
 // a score is over it by more than 8: weights then stay under e^8, which costs
 // no precision in fp32 and bf16, and most blocks do without a reduction over
@@ -491,14 +492,18 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
         for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
     }
     const float ref = m == -INFINITY ? 0.f : m;
-    unsigned hi[GP > 1 ? GP / 2 : 1], lo[GP > 1 ? GP / 2 : 1];   // two tokens each
+    constexpr int PAIRS = GP > 1 ? GP / 2 : 1;
+    unsigned hi[PAIRS], mid[PAIRS], lo[PAIRS];         // two tokens each
     if (GP == 1) {
       const float p = __builtin_amdgcn_exp2f((sc[0] - ref) * LOG2E);
       l += p;
       const __bf16 h1 = (__bf16)p;
-      const __bf16 l1 = (__bf16)(p - (float)h1);
+      const float rest = p - (float)h1;
+      const __bf16 m1 = (__bf16)rest;
+      const __bf16 l1 = (__bf16)(rest - (float)m1);
       const int odd = 16 * (c16 & 1);
       hi[0] = (unsigned)__builtin_bit_cast(unsigned short, h1) << odd;
+      mid[0] = (unsigned)__builtin_bit_cast(unsigned short, m1) << odd;
       lo[0] = (unsigned)__builtin_bit_cast(unsigned short, l1) << odd;
     } else {
 #pragma unroll
@@ -508,18 +513,21 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
         l += p0;
         l += p1;
         const bf16x2 h2 = bf16x2{(__bf16)p0, (__bf16)p1};
-        const bf16x2 l2 = bf16x2{(__bf16)(p0 - (float)h2[0]), (__bf16)(p1 - (float)h2[1])};
+        const float r0 = p0 - (float)h2[0], r1 = p1 - (float)h2[1];
+        const bf16x2 m2 = bf16x2{(__bf16)r0, (__bf16)r1};
+        const bf16x2 l2 = bf16x2{(__bf16)(r0 - (float)m2[0]), (__bf16)(r1 - (float)m2[1])};
         hi[i] = __builtin_bit_cast(unsigned, h2);
+        mid[i] = __builtin_bit_cast(unsigned, m2);
         lo[i] = __builtin_bit_cast(unsigned, l2);
       }
     }
     // tokens 2e, 2e + 1 are this lane's, or 0
-    u32x4 ph[2], pl[2];
+    u32x4 ph[2], pm[2], pl[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      constexpr int PAIRS = GP > 1 ? GP / 2 : 1;
       const bool own = GP > 1 ? part16 == e / PAIRS : part16 >> 1 == e;
       ph[e >> 2][e & 3] = own ? hi[e % PAIRS] : 0u;
+      pm[e >> 2][e & 3] = own ? mid[e % PAIRS] : 0u;
       pl[e >> 2][e & 3] = own ? lo[e % PAIRS] : 0u;
     }
 #pragma unroll
@@ -528,6 +536,7 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
       for (int e = 0; e < 2; ++e) {
         const bf16x8 v = v_frag(vr[i][2 * e], vr[i][2 * e + 1], vscale);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, ph[e]), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pm[e]), acc[i], 0, 0, 0);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pl[e]), acc[i], 0, 0, 0);
       }
   }
