@@ -248,10 +248,15 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
       for (int i = lane; i < D * (BLK / 4); i += 64) {
         const int t0 = i % (BLK / 4) * 4;
         if (t0 >= at) continue;
-        unsigned* c = reinterpret_cast<unsigned*>(codes + i / (BLK / 4) * BLK + t0);
-        // codes behind the new token stay as they were
-        const unsigned mask = at - t0 >= 4 ? 0xffffffffu : (1u << (8 * (at - t0))) - 1u;
-        *c = (rescale4(*c, ratio) & mask) | (*c & ~mask);
+        unsigned char* c = codes + i / (BLK / 4) * BLK + t0;
+        const unsigned r = rescale4(*reinterpret_cast<const unsigned*>(c), ratio);
+        // Of the word that the new token is in, the bytes before it alone: another
+        // lane writes its code, and those behind stay as they were.
+        if (at - t0 >= 4) {
+          *reinterpret_cast<unsigned*>(c) = r;
+        } else {
+          for (int j = 0; j < at - t0; ++j) c[j] = (unsigned char)(r >> (8 * j));
+        }
       }
     }
   }

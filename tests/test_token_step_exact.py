@@ -8,7 +8,7 @@ import torch
 
 from mi355 import ops
 
-from test_token_step import BF16, DEVICES, FP16, FP32, gen, gpu  # noqa: F401
+from test_token_step import BF16, DEVICES, FP16, FP32, Plain8, gen, gpu  # noqa: F401
 
 
 # --------------------------------------------------------------------------- #
@@ -46,3 +46,27 @@ def test_decode_attention_kv8_weights_have_32_bits(device, dtype, grp, d, length
     err = (out.double().cpu() - want).abs()
     tol = torch.finfo(dtype).eps / 2 * want + 2.0 ** -20
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+# --------------------------------------------------------------------------- #
+# append to the 8-bit cache                                                   #
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_kv8_append_one_grows_at_every_offset(device, dtype, d):
+    """One token at each position of a block, larger than all before it: the
+    old codes follow the new scale, the new code is there, and the codes behind
+    it keep their bytes, whichever of a word's bytes it takes."""
+    b, h = 64, 3
+    cache, plain = ops.KVCache8(b, h, 64, d, device=device), Plain8(b, h, 64, d)
+    old, new = (torch.randn(2, b, h, 64, d, generator=gen(j)).to(device, dtype) for j in (1, 2))
+    new = new[:, :, :, :1] * 40
+    ops.kv8_append(cache, old[0], old[1], 0)
+    plain.append(old[0], old[1], 0)
+    before = cache.k_scale.clone(), cache.v_scale.clone()
+    start = torch.arange(b, dtype=torch.int32, device=device)
+    ops.kv8_append(cache, new[0], new[1], start)
+    plain.append(new[0], new[1], start)
+    plain.same(cache)
+    assert bool((cache.k_scale > before[0]).all()) and bool((cache.v_scale > before[1]).all())
