@@ -12,10 +12,15 @@
 // lane (k = 128c + 32g + 8i + j) and x is read at the same k: no shuffle.
 //
 // Roundings: a converted weight has 2 significant bits and is exact in bf16 and
-// fp16.  Its exponent is taken relative to the row's largest group exponent
-// (put back in 32 bits at the end), so that fp16 holds it exactly down to
-// 2^-23 of the row's largest scale; below that it is less than half a unit of
-// an fp32 sum.  Sums are fp32; y is rounded once.
+// fp16 as far as their exponents reach.  So its exponent is taken relative to
+// the row's largest (put back in 32 bits at the end), in fp16 2^13 over it: from
+// 6 * 2^13 = 49152 down to 2^-14, half of the smallest scale, a row may span 26
+// octaves.  (Smaller ones would be exact as subnormal numbers, but a matrix
+// instruction loses bits of their sum: 6 units of 2^-24 of the sum of sizes at 35
+// octaves, 20 at 36, against 0.7 at up to 30.)  Groups of zeros do not count.
+// Rows that span more, which no quantizer of a trained weight makes, are summed
+// group by group in fp32 by the lanes that store them (far_outputs); their row
+// exponent is given as 255.  Sums are fp32; y is rounded once.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -32,6 +37,7 @@ typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 template <typename T> struct Frag;
 template <> struct Frag<__hip_bfloat16> {
   using vec = bf16x8;
+  static constexpr int BIAS = 0;      // octaves that weights stand over their row's scale
   template <int S> static DEVINL unsigned cvt2(unsigned codes, float scale) {
     return __builtin_bit_cast(unsigned,
                               __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, S));
@@ -42,6 +48,7 @@ template <> struct Frag<__hip_bfloat16> {
 };
 template <> struct Frag<__half> {
   using vec = f16x8;
+  static constexpr int BIAS = 13;
   template <int S> static DEVINL unsigned cvt2(unsigned codes, float scale) {
     return __builtin_bit_cast(unsigned,
                               __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, S));
@@ -62,15 +69,16 @@ DEVINL typename Frag<T>::vec decode8(unsigned codes, float scale) {
   return __builtin_bit_cast(typename Frag<T>::vec, r);
 }
 
-// 2^(e - row_e) as a float; differences under 2^-100 count as 2^-100
-DEVINL float group_scale(int e, int row_e) {
-  const int d = max(e - row_e, -100);
+// 2^(e - row_e + BIAS) as a float.  Of groups that are not all zeros the
+// difference is from -26 to 0 (or the row is FAR).
+template <typename T> DEVINL float group_scale(int e, int row_e) {
+  const int d = min(max(e - row_e, -100), 0) + Frag<T>::BIAS;
   return __builtin_bit_cast(float, (unsigned)(d + 127) << 23);
 }
 
-// 2^(e - 127); byte 0 is the subnormal 2^-127, 255 is no scale
-DEVINL float row_scale(int e) {
-  return __builtin_bit_cast(float, e ? (unsigned)e << 23 : 0x00400000u);
+// a sum of inputs times weights at group_scale, at the row's scale
+template <typename T> DEVINL float at_row_scale(float sum, int row_e) {
+  return __builtin_amdgcn_ldexpf(sum, row_e - 127 - Frag<T>::BIAS);
 }
 
 struct Args {
@@ -79,11 +87,47 @@ struct Args {
   long ldx;
 };
 
+constexpr int FAR = 255;                // the row exponent of rows without one scale for all
+
+// One output of such a row: a sum in fp32 for each group, its scale, their sum.
+template <typename T> DEVINL float far_output(const T* x, const Args& a, int m, int n) {
+  const unsigned char* codes = a.codes + (long)n * (a.K >> 1);
+  const unsigned char* exps = a.exps + (long)n * (a.K >> 5);
+  x += m * a.ldx;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < a.K; k += 32) {
+    float s = 0.f;
+#pragma unroll 1
+    for (int i = k; i < k + 32; i += 8) {
+      const unsigned c = *reinterpret_cast<const unsigned*>(codes + (i >> 1));
+      const VecT<T, 8> v = vload<T, 8>(x + i);
+      auto two = [&](auto w, int at) {
+        s = fmaf(DT<T>::to_f32(v.data[at]), w[0], s);
+        s = fmaf(DT<T>::to_f32(v.data[at + 1]), w[1], s);
+      };
+      two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0), 0);
+      two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1), 2);
+      two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2), 4);
+      two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3), 6);
+    }
+    const int e = exps[k >> 5];
+    sum += e == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(s, e - 127);
+  }
+  return sum;
+}
+
+// The outputs [m0, m1) of row n, by the lane that stored them.
+template <typename T> DEVINL void far_outputs(const T* x, T* y, const Args& a, int m0, int m1, int n) {
+#pragma unroll 1
+  for (int m = m0; m < min(m1, a.M); ++m) y[(long)m * a.N + n] = DT<T>::from_f32(far_output(x, a, m, n));
+}
+
 // The block's waves hold sums over parts of K, each for the 16 * NT outputs from
 // n0 - lane%16 on: added through LDS in wave order (the same sum every time) and
 // stored.  D layout: column n = lane%16, row m = 4*(lane/16) + r.
 template <typename T, int NT, int WAVES>
-DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, T* y, const Args& a) {
+DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, const T* x, T* y, const Args& a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int u = 0; u < NT; ++u) part[wave][u][lane] = acc[u];
@@ -98,12 +142,13 @@ DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, T* y, con
       for (int r = 0; r < 4; ++r) s[r] += p[r];
     }
     if (n >= a.N) continue;
-    const float back = row_scale(a.row_exp[n]);
+    const int row_e = a.row_exp[n];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = 4 * (lane >> 4) + r;
-      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(s[r] * back);
+      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(at_row_scale<T>(s[r], row_e));
     }
+    if (row_e == FAR) far_outputs(x, y, a, 4 * (lane >> 4), 4 * (lane >> 4) + 4, n);
   }
 }
 
@@ -166,13 +211,13 @@ w4_few_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
     if (k0 + WAVES * 128 < a.K) next = load(k0 + WAVES * 128);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const float scale = group_scale(p.e[u], row_e[u]);
+      const float scale = group_scale<T>(p.e[u], row_e[u]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         acc[u] = Frag<T>::mfma(__builtin_bit_cast(vec, p.x[i]), decode8<T>(p.w[u][i], scale), acc[u]);
     }
   }
-  add_waves<T, NT, WAVES>(part, acc, n0, y, a);
+  add_waves<T, NT, WAVES>(part, acc, n0, x, y, a);
 }
 
 // Elements of a row of x in LDS: zeros behind K as far as a wave's pieces reach
@@ -249,7 +294,7 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
       const int k = k0 + 128 * j + 32 * g;
       float scale[NT];
 #pragma unroll
-      for (int u = 0; u < NT; ++u) scale[u] = group_scale(p.e[j][u], row_e[u]);
+      for (int u = 0; u < NT; ++u) scale[u] = group_scale<T>(p.e[j][u], row_e[u]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const vec xf = *reinterpret_cast<const vec*>(xrow + k + 8 * i);
@@ -259,7 +304,7 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
       }
     }
   }
-  add_waves<T, NT, WAVES>(part, acc, n0, y, a);
+  add_waves<T, NT, WAVES>(part, acc, n0, x, y, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -352,7 +397,7 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
     u32x4 w[NT];
     float scale[NT];
 #pragma unroll
-    for (int u = 0; u < NT; ++u) { w[u] = now.w[u] & keep; scale[u] = group_scale(now.e[u], row_e[u]); }
+    for (int u = 0; u < NT; ++u) { w[u] = now.w[u] & keep; scale[u] = group_scale<T>(now.e[u], row_e[u]); }
     load(now, k0 + 2 * KC);
     const T* row = &lds[buf][g * PLANE + (wm * 16 * MT + c16) * LD];
 #pragma unroll
@@ -383,7 +428,6 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
   for (int u = 0; u < NT; ++u) {
     const int n = n0 + 16 * u;
     if (n >= a.N) continue;
-    const float back = row_scale(row_e[u]);
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -391,21 +435,32 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
         const int m = m_at + wm * 16 * MT + 16 * t + 4 * g + r;
         if (m >= a.M) continue;
         if (part) part[((long)blockIdx.z * a.M + m) * a.N + n] = acc[t][u][r];
-        else y[(long)m * a.N + n] = DT<T>::from_f32(acc[t][u][r] * back);
+        else y[(long)m * a.N + n] = DT<T>::from_f32(at_row_scale<T>(acc[t][u][r], row_e[u]));
       }
+  }
+  bool far = false;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) far |= row_e[u] == FAR;
+  if (far && !part) {                               // w4_add_parts makes them otherwise
+#pragma unroll 1
+    for (int i = 0; i < NT * MT; ++i) {
+      const int n = n0 + 16 * (i / MT), m = m_at + wm * 16 * MT + 16 * (i % MT) + 4 * g;
+      if (n < a.N && a.row_exp[n] == FAR) far_outputs(x, y, a, m, m + 4, n);
+    }
   }
 }
 
 // The sum over parts of K, in their order, and the rows' scales.
 template <typename T>
 __global__ void __launch_bounds__(256)
-w4_add_parts(const float* __restrict__ part, T* __restrict__ y, int parts, Args a) {
+w4_add_parts(const T* __restrict__ x, const float* __restrict__ part, T* __restrict__ y, int parts, Args a) {
   const long mn = (long)a.M * a.N, i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= mn) return;
   float s = 0.f;
 #pragma unroll 4
   for (int p = 0; p < parts; ++p) s += part[p * mn + i];
-  y[i] = DT<T>::from_f32(s * row_scale(a.row_exp[i % a.N]));
+  const int m = i / a.N, n = i - (long)m * a.N, row_e = a.row_exp[n];
+  y[i] = DT<T>::from_f32(row_e == FAR ? far_output(x, a, m, n) : at_row_scale<T>(s, row_e));
 }
 
 }  // namespace
@@ -460,8 +515,8 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
       float* p = parts > 1 ? part.data_ptr<float>() : nullptr;
       launch(kernel, grid, threads, 0, p, (int)run);
       if (parts > 1)
-        hipLaunchKernelGGL(w4_add_parts<T>, dim3(up(M * N, 256)), dim3(256), 0, stream, p,
-                           (T*)y.data_ptr(), (int)parts, a);
+        hipLaunchKernelGGL(w4_add_parts<T>, dim3(up(M * N, 256)), dim3(256), 0, stream,
+                           (const T*)x.data_ptr(), p, (T*)y.data_ptr(), (int)parts, a);
     };
     const auto tiles = [&](long t) { return dim3(up(M, t), up(N, t)); };
     const auto count = [](dim3 d) { return (long)d.x * d.y; };

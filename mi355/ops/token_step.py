@@ -45,6 +45,8 @@ class W4Weight(torch.nn.Module):
     ``codes`` (N, K/2) uint8, ``exps`` (N, K/32) uint8; K a multiple of 32.
     An exponent of 255 is no scale (the format's NaN): its row's outputs are
     not finite.  The buffers are read as they lie: nothing is laid out anew.
+    ``row_exp`` (N,) is made from them, here and when a state is loaded: they
+    are not to be written over otherwise.
     """
 
     GROUP = 32
@@ -60,8 +62,12 @@ class W4Weight(torch.nn.Module):
             raise ValueError(f"codes on {codes.device}, exponents on {exps.device}")
         self.register_buffer("codes", codes.contiguous())
         self.register_buffer("exps", exps.contiguous())
-        # the row's largest group exponent: what the kernel scales against
-        self.register_buffer("row_exp", exps.amax(1) if len(exps) else exps.new_empty(0))
+        self.register_buffer("row_exp", torch_ref.w4_row_exp(codes, exps))
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        with torch.no_grad():
+            self.row_exp.copy_(torch_ref.w4_row_exp(self.codes, self.exps))
 
     @property
     def shape(self) -> torch.Size:
@@ -69,7 +75,11 @@ class W4Weight(torch.nn.Module):
 
     def rows(self, start: int, stop: int) -> "W4Weight":
         """Output rows [start, stop) as a weight that shares the buffers."""
-        return W4Weight(self.codes[start:stop], self.exps[start:stop])
+        part = W4Weight.__new__(W4Weight)
+        torch.nn.Module.__init__(part)
+        for name in ("codes", "exps", "row_exp"):
+            part.register_buffer(name, self._buffers[name][start:stop])
+        return part
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return torch_ref.w4_dequantize(self.codes, self.exps).to(dtype)
@@ -101,7 +111,9 @@ def linear_w4(x: torch.Tensor, w: W4Weight) -> torch.Tensor:
     """``x @ w.T`` for x (..., K) in bf16 or fp16: sums in 32 bits, one rounding
     at the end.  Any number of rows; made for the few that decoding has.  The
     largest scale of a row of w is multiplied in after its sum: sums of x times
-    codes have to stay in fp32's range (inputs under 2^125 / K do)."""
+    codes have to stay in fp32's range (inputs under 2^125 / K and over 2^-99
+    do).  A row of w whose scales lie over 26 octaves apart, groups of zeros not
+    counted, is right too, but slow: its groups are summed one by one."""
     if x.is_cuda and _use_hip(x):
         b = w._buffers
         return _load_ext().w4_linear(x, b["codes"], b["exps"], b["row_exp"])

@@ -135,15 +135,29 @@ def seg_postprocess(logits: torch.Tensor, size) -> torch.Tensor:
 # 4-bit weights                                                               #
 # --------------------------------------------------------------------------- #
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+W4_SPAN = 26        # octaves between scales that weights in 16 bits hold (csrc/kernels/w4_linear.hip)
 
 
-def w4_dequantize(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
-    """(N, K/2) codes and (N, K/32) exponents -> fp32 (N, K)."""
+def w4_dequantize(codes: torch.Tensor, exps: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
+    """(N, K/2) codes and (N, K/32) exponents -> (N, K); a byte of 255 is NaN."""
     n, half = codes.shape
-    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
+    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device, dtype=dtype)
     nibbles = torch.stack([codes & 15, codes >> 4], -1).view(n, half // 16, 32)
-    scale = torch.ldexp(torch.ones((), device=codes.device), exps.int() - 127)
+    scale = torch.ldexp(torch.ones((), device=codes.device, dtype=dtype), exps.int() - 127)
+    scale = torch.where(exps == 255, math.nan, scale)
     return (table[nibbles.int()] * scale[..., None]).view(n, 2 * half)
+
+
+def w4_row_exp(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    """(N,) uint8, what the kernels scale a row against: its largest exponent
+    byte of a group that holds more than zeros; 255 where those of the row lie
+    over W4_SPAN apart, or one is no scale: such a row is summed group by
+    group."""
+    there = (codes & 0x77).view(*exps.shape, 16).amax(-1) > 0
+    most = torch.where(there, exps, 0).amax(1)
+    least = torch.where(there, exps, 255).amin(1)
+    apart = (most.int() - least.int() > W4_SPAN) | (exps == 255).any(1)
+    return torch.where(apart, 255, most).to(torch.uint8)
 
 
 def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -175,8 +189,8 @@ def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def linear_w4(x: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
-    acc = x.dtype if x.dtype == torch.float64 else torch.float32
-    return torch.matmul(x.to(acc), w4_dequantize(codes, exps).to(acc).t()).to(x.dtype)
+    # in 64 bits: 6 * 2^127 is a weight, and over fp32's range
+    return torch.matmul(x.double(), w4_dequantize(codes, exps, torch.float64).t()).to(x.dtype)
 
 
 # --------------------------------------------------------------------------- #

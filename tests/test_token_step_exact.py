@@ -8,7 +8,153 @@ import torch
 
 from mi355 import ops
 
-from test_token_step import BF16, DEVICES, FP16, FP32, Plain8, gen, gpu  # noqa: F401
+from test_token_step import BF16, DEVICES, FP16, FP32, Plain8, gen, gpu, w4_values  # noqa: F401
+
+
+# --------------------------------------------------------------------------- #
+# 4-bit weights                                                               #
+# --------------------------------------------------------------------------- #
+# every kernel, of few rows and of many: x in LDS (of both forms), x from the
+# caches (of one, two and four tiles), tiles of 128, of 64 with and without
+# shared K, of 32
+W4_SHAPES = [(1, 40, 96), (2, 24, 512), (8, 40, 416), (2, 16390, 96), (8, 40, 4640), (12, 40, 160), (8, 8200, 4640),
+             (12, 8210, 160), (130, 8200, 96), (70, 70, 4128), (129, 2700, 128), (40, 40, 416)]
+SPANS = [0, 20, 22, 23, 24, 30, 35, 36, 37, 38, 50, 60, 99, 101, 134]     # octaves between a row's scales
+
+
+def check_group_sums(x, w, y):
+    """Against 64 bits, with what fp32 sums of the terms that are there can
+    lose (terms that are 0 add no error) and y's own rounding: half a step, of
+    the subnormal numbers where y is one."""
+    ref_w = w4_values(w.codes, w.exps)
+    x64 = x.double().cpu()
+    ref, size = x64 @ ref_w.t(), x64.abs() @ ref_w.abs().t()
+    terms = int((x64 != 0).sum(1).max()) + 4
+    info = torch.finfo(y.dtype)
+    tol = info.eps / 2 * ref.abs() + terms * 2.0 ** -24 * size + info.smallest_normal * info.eps / 2
+    err = (y.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), (float((err / tol).max()), (err > tol).nonzero()[:5].tolist())
+
+
+def far_w4(n, k, device, big, empty=False, low=120):
+    """Rows whose group `big` has a scale SPANS[row] octaves over the others';
+    with `empty` all codes of that group are 0 or -0."""
+    g = gen(n + k)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    exps = torch.full((n, k // 32), low, dtype=torch.uint8)
+    exps[:, big] = low + torch.tensor([SPANS[i % len(SPANS)] for i in range(n)], dtype=torch.uint8)
+    if empty:
+        codes[:, 16 * big:16 * big + 16] &= 0x88
+    return ops.W4Weight(codes.to(device), exps.to(device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", W4_SHAPES)
+def test_linear_w4_small_scales_beside_large_ones(device, dtype, m, n, k):
+    """What the small scales of a row contribute is there in full where the
+    group of the large scale contributes nothing: its inputs are 0, or its
+    codes."""
+    if device == "cpu" and m * n * k > 10 ** 7:
+        n = n % 509
+    groups = k // 32
+    for big in {0, groups - 1}:
+        x = torch.randn(m, k, generator=gen(m)).to(device, dtype)
+        w = far_w4(n, k, device, big, empty=True)
+        check_group_sums(x, w, ops.linear_w4(x, w))
+        w = far_w4(n, k, device, big)
+        x[:, 32 * big:32 * big + 32] = 0
+        check_group_sums(x, w, ops.linear_w4(x, w))
+        # one group alone
+        only = torch.zeros_like(x)
+        at = 32 * ((big + 1) % groups)
+        only[:, at:at + 32] = x[:, at:at + 32]
+        check_group_sums(only, w, ops.linear_w4(only, w))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_linear_w4_each_distance(device, dtype):
+    """Rows with a scale for every distance from 0 to 130 octaves, x in one
+    group at a time; dense x; an infinity in the group of the smallest scale."""
+    k = 32 * 131
+    codes = torch.randint(0, 256, (6, k // 2), generator=gen(1), dtype=torch.uint8)
+    exps = torch.stack([torch.arange(131).flip(0) + 100, torch.arange(131) + 5,
+                        torch.randperm(131, generator=gen(2)) + 110, torch.full((131,), 121),
+                        torch.arange(131) % 37 + 100, torch.arange(131) % 38 + 100]).to(torch.uint8)
+    w = ops.W4Weight(codes.to(device), exps.to(device))
+    x = torch.randn(131, k, generator=gen(3)) * torch.eye(131).repeat_interleave(32, 1)
+    if dtype == FP16:
+        # outputs stay in range where x * scale does
+        x = torch.where(x.abs() * 200 * 2.0 ** (exps.amax(0).float() - 127).repeat_interleave(32) < 60000, x, 0.0)
+    x = x.to(device, dtype)
+    y = ops.linear_w4(x, w)
+    check_group_sums(x, w, y)
+    for rows in (1, 7, 16, 40):
+        check_group_sums(x[:rows], w, ops.linear_w4(x[:rows], w))
+        check_group_sums(x[-rows:], w, ops.linear_w4(x[-rows:], w))
+    dense = torch.randn(3, k, generator=gen(4)).to(device, BF16)
+    check_group_sums(dense, w, ops.linear_w4(dense, w))
+    ones = ops.W4Weight(torch.full_like(w.codes, 0x22), w.exps)
+    x = torch.zeros(2, k, device=device, dtype=dtype)
+    x[0, k - 5] = math.inf
+    x[1, 3] = -math.inf
+    y = ops.linear_w4(x, ones)
+    assert bool((y[0] == math.inf).all()) and bool((y[1] == -math.inf).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("span", [25, 26, 27, 28])
+def test_linear_w4_where_rows_are_summed_by_groups(device, dtype, span):
+    """On both sides of the border, all groups of one row alike."""
+    k = 160
+    w = ops.W4Weight(*(t.to(device) for t in (
+        torch.randint(0, 256, (300, k // 2), generator=gen(span), dtype=torch.uint8),
+        torch.tensor([120, 120 + span, 121, 120 + span // 2, 120], dtype=torch.uint8).repeat(300, 1))))
+    assert bool((w.row_exp == (255 if span > 26 else 120 + span)).all())
+    x = torch.randn(140, k, generator=gen(5)).to(device, dtype)
+    for keep in ((0,), (4,), (0, 4), (2, 4), (3,), (0, 2, 3, 4)):
+        part = torch.zeros_like(x)
+        for at in keep:
+            part[:, 32 * at:32 * at + 32] = x[:, 32 * at:32 * at + 32]
+        if dtype == FP16 and 3 in keep:
+            part = part / 4
+        for rows in (1, 9, 17, 140):
+            check_group_sums(part[:rows], w, ops.linear_w4(part[:rows], w))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", W4_SHAPES)
+def test_linear_w4_no_scale(device, dtype, m, n, k):
+    """An exponent byte of 255, over codes of 0 as well, makes its own row's
+    outputs not finite and no other's."""
+    if device == "cpu" and m * n * k > 10 ** 7:
+        n = n % 509
+    codes = torch.full((n, k // 2), 0x22, dtype=torch.uint8)
+    exps = torch.full((n, k // 32), 127, dtype=torch.uint8)
+    codes[3], exps[3, k // 32 - 1] = 0, 255
+    exps[n - 1, 0] = 255
+    y = ops.linear_w4(torch.ones(m, k, device=device, dtype=dtype), ops.W4Weight(codes.to(device), exps.to(device)))
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[[3, n - 1]] = True
+    assert torch.equal(~y.isfinite().cpu(), bad.expand(m, n))
+    assert bool((y.cpu()[:, ~bad].double() == torch.tensor(float(k)).to(dtype).double()).all())
+
+
+def test_w4_weight_loads_and_slices():
+    """What is made from the exponents follows a load, and slices share it."""
+    a, b = far_w4(30, 96, "cpu", 0), far_w4(30, 96, "cpu", 2, empty=True)
+    before = a.row_exp.clone()
+    state = b.state_dict()
+    state["row_exp"] = torch.zeros_like(state["row_exp"])           # as if another rule had made it
+    a.load_state_dict(state)
+    assert torch.equal(a.row_exp, b.row_exp) and not torch.equal(a.row_exp, before)
+    part = b.rows(7, 20)
+    assert part.shape == (13, 96) and torch.equal(part.row_exp, b.row_exp[7:20])
+    for name in ("codes", "exps"):
+        assert getattr(part, name).data_ptr() == getattr(b, name)[7:].data_ptr()
 
 
 # --------------------------------------------------------------------------- #
