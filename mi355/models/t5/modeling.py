@@ -684,8 +684,14 @@ class T5ForConditionalGeneration(nn.Module):
         # generations could emit EOS mid-sequence followed by garbage that
         # survives skip_special_tokens decoding.
         eos = cfg.eos_token_id if eos_token_id is None else eos_token_id
+        # What the capture bakes in: shapes, tokens, options, and where each
+        # weight lies.  Weights written in place are followed; ones that were
+        # cast, moved or replaced are somewhere else.
         key = (b, input_ids.shape[1], max_new_tokens, str(dev), eos, kv8,
-               tuple(sampling.values()) if sampling is not None else None)
+               tuple(sampling.values()) if sampling is not None else None,
+               cfg.decoder_start_token_id, cfg.pad_token_id, cfg.tie_word_embeddings,
+               tuple((w.data_ptr(), w.dtype) for m in (self.decoder, self.lm_head)
+                     for w in (*m.parameters(), *m.buffers())))
         state = getattr(self, "_gen_graph", None)
         kpad = _kpad_from_mask(attention_mask)
         enc = self.encoder(input_ids=input_ids, kpad=kpad)
