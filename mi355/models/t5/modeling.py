@@ -684,6 +684,9 @@ class T5ForConditionalGeneration(nn.Module):
         # generations could emit EOS mid-sequence followed by garbage that
         # survives skip_special_tokens decoding.
         eos = cfg.eos_token_id if eos_token_id is None else eos_token_id
+        state = getattr(self, "_gen_graph", None)
+        kpad = _kpad_from_mask(attention_mask)
+        enc = self.encoder(input_ids=input_ids, kpad=kpad)
         # What the capture bakes in: shapes, tokens, options, and where each
         # weight lies.  Weights written in place are followed; ones that were
         # cast, moved or replaced are somewhere else.
@@ -692,9 +695,8 @@ class T5ForConditionalGeneration(nn.Module):
                cfg.decoder_start_token_id, cfg.pad_token_id, cfg.tie_word_embeddings,
                tuple((w.data_ptr(), w.dtype) for m in (self.decoder, self.lm_head)
                      for w in (*m.parameters(), *m.buffers())))
-        state = getattr(self, "_gen_graph", None)
-        kpad = _kpad_from_mask(attention_mask)
-        enc = self.encoder(input_ids=input_ids, kpad=kpad)
+        attn0 = self.decoder.block[0].layer[0].SelfAttention
+        full_bias = attn0.compute_bias(max_new_tokens, max_new_tokens, dev).float()
         if state is None or state["key"] != key or (kpad is None) != (state["kpad"] is None):
             # build static buffers and capture the 128-step decode loop
             caches = self._decode_caches(enc, b, max_new_tokens, dev, dt, kv8)
@@ -702,12 +704,7 @@ class T5ForConditionalGeneration(nn.Module):
             enc_static = enc.clone()
             kpad_static = kpad.clone() if kpad is not None else None
             out_tokens = torch.zeros(b, max_new_tokens, device=dev, dtype=torch.long)
-            attn0 = self.decoder.block[0].layer[0].SelfAttention
-            full_bias = attn0.compute_bias(max_new_tokens, max_new_tokens, dev).float()
-            # the 8-bit path reads the fp32 row in place, behind the length too
-            bias_steps = [full_bias[:, :, t:t + 1] if kv8 else
-                          full_bias[:, :, t:t + 1, :t + 1].contiguous()
-                          for t in range(max_new_tokens)]
+            bias_static = full_bias.clone()
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
@@ -716,8 +713,10 @@ class T5ForConditionalGeneration(nn.Module):
                 for i in range(len(caches)):
                     caches[i]["self"]["len"] = 0
                 for t in range(max_new_tokens):
-                    dec = self._decode_step(tok, enc_static, kpad_static, caches,
-                                            t, bias_steps[t] if kv8 else bias_steps[t].to(dt))
+                    # the 8-bit path reads the fp32 row in place, behind the length too
+                    bias_t = bias_static[:, :, t:t + 1] if kv8 else \
+                        bias_static[:, :, t:t + 1, :t + 1].to(dt).contiguous()
+                    dec = self._decode_step(tok, enc_static, kpad_static, caches, t, bias_t)
                     if cfg.tie_word_embeddings:
                         dec = dec * (self.model_dim**-0.5)
                     logits = self._lm_logits(dec[:, -1])
@@ -728,10 +727,11 @@ class T5ForConditionalGeneration(nn.Module):
                     tok = nxt.unsqueeze(1)
             state = {"key": key, "graph": g, "enc": enc_static, "kpad": kpad_static,
                      "caches": caches, "out": out_tokens, "u": u_static,
-                     "bias": bias_steps}
+                     "bias": bias_static}
             self._gen_graph = state
         # refresh the static inputs, reset self-cache lengths, replay
         state["enc"].copy_(enc)
+        state["bias"].copy_(full_bias)
         if kpad is not None:
             state["kpad"].copy_(kpad)
         if u is not None:

@@ -72,3 +72,21 @@ def test_captured_loop_keeps_its_graph():
         for w in m.parameters():
             w.mul_(1.01)
     assert torch.equal(*both(m)) and m._gen_graph is state
+
+
+@gpu
+@pytest.mark.parametrize("options", [dict(), dict(kv_cache_dtype="fp8")])
+def test_captured_loop_follows_the_position_bias(options):
+    """The bias of the relative positions is the present one, not that of the
+    capture."""
+    m = model("cuda")
+    assert torch.equal(*both(m, **options))
+    state = m._gen_graph
+    weight = m.decoder.block[0].layer[0].SelfAttention.relative_attention_bias.weight
+    before = both(m, **options)[0]
+    for seed in (3, 4):
+        with torch.no_grad():
+            weight.copy_(torch.randn(weight.shape, generator=torch.Generator().manual_seed(seed)) * 30)
+        out = both(m, **options)
+        assert torch.equal(*out) and not torch.equal(out[0], before)
+    assert m._gen_graph is state
