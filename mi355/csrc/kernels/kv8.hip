@@ -239,24 +239,36 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
   const float inv = 1.f / scale;                  // exact: a power of two
   if (at > 0 && scale > old) {
     const float ratio = old * inv;
+    const int t0 = lane % 16 * 4;                 // this lane's word of every fourth row of V
     if (!is_v) {
       for (int i = lane * 4; i < at * D; i += 256) {
         unsigned* c = reinterpret_cast<unsigned*>(codes + i);
         *c = rescale4(*c, ratio);
       }
     } else {
-      for (int i = lane; i < D * (BLK / 4); i += 64) {
-        const int t0 = i % (BLK / 4) * 4;
-        if (t0 >= at) continue;
-        unsigned char* c = codes + i / (BLK / 4) * BLK + t0;
-        const unsigned r = rescale4(*reinterpret_cast<const unsigned*>(c), ratio);
-        // Of the word that the new token is in, the bytes before it alone: another
-        // lane writes its code, and those behind stay as they were.
-        if (at - t0 >= 4) {
-          *reinterpret_cast<unsigned*>(c) = r;
-        } else {
-          for (int j = 0; j < at - t0; ++j) c[j] = (unsigned char)(r >> (8 * j));
+      // whole words before the new token's
+      if (t0 + 4 <= at) {
+        unsigned w[D / 4];
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) w[i] = *reinterpret_cast<const unsigned*>(codes + (lane / 16 + 4 * i) * BLK + t0);
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+          *reinterpret_cast<unsigned*>(codes + (lane / 16 + 4 * i) * BLK + t0) = rescale4(w[i], ratio);
+      }
+      // the new token's word, by the lane that has its code: bytes before it
+      // follow the scale, those behind it stay
+      if (const int byte = at & 3) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          if (d0 + u >= D) break;
+          unsigned* c = reinterpret_cast<unsigned*>(codes + (d0 + u) * BLK + at - byte);
+          const unsigned before = (1u << (8 * byte)) - 1u, here = 0xffu << (8 * byte);
+          const unsigned was = *c;
+          *c = (rescale4(was, ratio) & before) | (unsigned)encode1(x[u] * inv) << (8 * byte) |
+               (was & ~(before | here));
         }
+        if (lane == 0) *scale_at = scale;
+        return;
       }
     }
   }
