@@ -302,7 +302,10 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
 //
 // P is split into three bf16 numbers, p = hi + mid + lo, 8 significant bits
 // each: all of its 24.  (With two a weight is off by up to 2^-18, and ten times
-// as many outputs land a step beside the nearest one.)  The reference m that is
+// as many outputs land a step beside the nearest one.)  A column's other weights
+// are 0, so mid and lo go there, one column and two columns of the same head
+// further: up to 4 heads take one matrix instruction a tile for all three, up to
+// 8 two, 16 three.  The reference m that is
 // subtracted in the exponent is raised, and what was summed rescaled, only when
 // a score is over it by more than 8: weights then stay under e^8, which costs
 // no precision in fp32 and bf16, and most blocks do without a reduction over
@@ -370,16 +373,19 @@ struct AttnArgs {
 constexpr int MAX_SPLIT = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// x of the lane that is BY away, round a row of 16
+template <int BY, typename X> DEVINL X turned(X x) {
+  static_assert(BY > 0 && BY < 16 && sizeof(X) == 4, "");
+  return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + BY,
+                                                           0xf, 0xf, false));
+}
+
 // op over the columns of a head: lanes of a row of 16 that are GP apart
 template <int GP, typename Op> DEVINL float over_columns(float x, Op op) {
-  auto turned = [](float v, auto by) {            // from the lane `by` on, round the row
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-        0, __builtin_bit_cast(int, v), 0x120 + by, 0xf, 0xf, false));
-  };
-  if (GP < 16) x = op(x, turned(x, std::integral_constant<int, 8>()));
-  if (GP < 8) x = op(x, turned(x, std::integral_constant<int, 4>()));
-  if (GP < 4) x = op(x, turned(x, std::integral_constant<int, 2>()));
-  if (GP < 2) x = op(x, turned(x, std::integral_constant<int, 1>()));
+  if (GP < 16) x = op(x, turned<8>(x));
+  if (GP < 8) x = op(x, turned<4>(x));
+  if (GP < 4) x = op(x, turned<2>(x));
+  if (GP < 2) x = op(x, turned<1>(x));
   return x;
 }
 
@@ -403,6 +409,9 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
   const int split = blockIdx.y;
   const int q0 = blockIdx.z * GP;                      // first query head of the group
   const int col = c16 % GP, part16 = c16 / GP;         // this lane's head, and its tokens
+  // the tokens whose mid and lo it takes
+  const int mid_part = GP <= 8 ? turned<GP <= 8 ? GP : 1>(part16) : part16;
+  const int lo_part = GP <= 4 ? turned<GP <= 4 ? 2 * GP : 1>(part16) : part16;
   const bool col_ok = q0 + col < a.G;
   const int hq = h * a.G + q0 + (col_ok ? col : 0);
   const int len = min(max(lengths.at(b), 0), a.max_len);
@@ -538,23 +547,36 @@ kv8_attn_kernel(const T* __restrict__ q, long qsb, long qsh, const unsigned char
         lo[i] = __builtin_bit_cast(unsigned, l2);
       }
     }
-    // tokens 2e, 2e + 1 are this lane's, or 0
-    u32x4 ph[2], pm[2], pl[2];
+    // The column's weights, tokens 2e and 2e + 1 in a word: hi of this lane's
+    // tokens; mid and lo of those of the head's next two columns, as far as it has
+    // as many, else in operands of their own.
+    if (GP <= 8) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) mid[i] = turned<GP <= 8 ? GP : 1>(mid[i]);
+    }
+    if (GP <= 4) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) lo[i] = turned<GP <= 4 ? 2 * GP : 1>(lo[i]);
+    }
+    u32x4 p[1 + (GP > 8) + (GP > 4)][2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool own = GP > 1 ? part16 == e / PAIRS : part16 >> 1 == e;
-      ph[e >> 2][e & 3] = own ? hi[e % PAIRS] : 0u;
-      pm[e >> 2][e & 3] = own ? mid[e % PAIRS] : 0u;
-      pl[e >> 2][e & 3] = own ? lo[e % PAIRS] : 0u;
+      const auto of = [&](int part, const unsigned (&w)[PAIRS]) {
+        return (GP > 1 ? part == e / PAIRS : part >> 1 == e) ? w[e % PAIRS] : 0u;
+      };
+      const unsigned h = of(part16, hi), m_ = of(mid_part, mid), l_ = of(lo_part, lo);
+      p[0][e >> 2][e & 3] = GP <= 4 ? h | m_ | l_ : GP <= 8 ? h | m_ : h;
+      if (GP > 8) p[1][e >> 2][e & 3] = m_;
+      if (GP > 4) p[GP > 8 ? 2 : 1][e >> 2][e & 3] = l_;
     }
 #pragma unroll
     for (int i = 0; i < DT16; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const bf16x8 v = v_frag(vr[i][2 * e], vr[i][2 * e + 1], vscale);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, ph[e]), acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pm[e]), acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, pl[e]), acc[i], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(p) / sizeof(p[0])); ++j)
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, p[j][e]), acc[i], 0, 0, 0);
       }
   }
   const auto sum = [](float x, float y) { return x + y; };
