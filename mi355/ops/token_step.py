@@ -65,9 +65,13 @@ class W4Weight(torch.nn.Module):
         self.register_buffer("row_exp", torch_ref.w4_row_exp(codes, exps))
 
     def _load_from_state_dict(self, *args, **kwargs):
+        row_exp = self.row_exp
         super()._load_from_state_dict(*args, **kwargs)
-        with torch.no_grad():
-            self.row_exp.copy_(torch_ref.w4_row_exp(self.codes, self.exps))
+        fresh = torch_ref.w4_row_exp(self.codes, self.exps)
+        if self.row_exp is row_exp:
+            row_exp.copy_(fresh)
+        else:                                   # the caller's tensor, of an assigning load
+            self.row_exp = fresh
 
     @property
     def shape(self) -> torch.Size:

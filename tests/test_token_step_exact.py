@@ -157,6 +157,18 @@ def test_w4_weight_loads_and_slices():
         assert getattr(part, name).data_ptr() == getattr(b, name)[7:].data_ptr()
 
 
+def test_w4_weight_leaves_a_loaded_state_alone():
+    """A load, an assigning one too, writes nothing into what it was given."""
+    for assign in (False, True):
+        a, b = far_w4(30, 96, "cpu", 0), far_w4(30, 96, "cpu", 2, empty=True)
+        state = {k: v.clone() for k, v in b.state_dict().items()}
+        state["row_exp"].zero_()
+        at = a.row_exp.data_ptr()
+        a.load_state_dict(state, assign=assign)
+        assert torch.equal(a.row_exp, b.row_exp) and not bool(state["row_exp"].any())
+        assert assign or a.row_exp.data_ptr() == at                  # a captured graph reads it there
+
+
 # --------------------------------------------------------------------------- #
 # attention over the 8-bit cache                                              #
 # --------------------------------------------------------------------------- #
