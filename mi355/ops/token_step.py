@@ -100,12 +100,13 @@ class W4Weight(torch.nn.Module):
 
 @torch.no_grad()
 def quantize_w4(weight: torch.Tensor) -> W4Weight:
-    """The nearest :class:`W4Weight` of a finite (N, K) weight: for each group
-    of 32 inputs that power of two, of the two next to amax/6, whose rounded
-    codes are off by the smaller sum of squares.  Waits for the device once, to
-    refuse what is not finite."""
+    """The nearest :class:`W4Weight` of an (N, K) weight that is finite in fp32:
+    for each group of 32 inputs that power of two, of the two next to amax/6,
+    whose rounded codes are off by the smaller sum of squares.  Waits for the
+    device once, to refuse what is not finite."""
     if weight.dim() != 2 or weight.shape[1] % W4Weight.GROUP or not weight.shape[1]:
         raise ValueError(f"quantize_w4 takes (N, K) with K a multiple of 32, got {tuple(weight.shape)}")
+    weight = weight.float()
     if not torch.isfinite(weight).all():
         raise ValueError("quantize_w4 takes a finite weight")
     return W4Weight(*torch_ref.w4_quantize(weight))

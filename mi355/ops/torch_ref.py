@@ -171,13 +171,15 @@ def w4_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     edges = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device=w.device)
     table = torch.tensor(E2M1, device=w.device)
     best = None
+    e = e.clamp(-126, 126)
     for less in (0, 1):
-        ee = (e - less).clamp(-126, 126)
+        ee = (e - less).clamp(min=-126)
         scaled = torch.ldexp(w, -ee)
         up = torch.bucketize(scaled.abs(), edges, right=True)    # ties up
         down = torch.bucketize(scaled.abs(), edges)              # ties down
         code = torch.where(up % 2 == 0, up, down)
-        err = ((table[code] - scaled.abs()) * torch.ldexp(torch.ones_like(amax), ee)).square().sum(-1, keepdim=True)
+        # at the upper scale: squares of the weights themselves may leave fp32's range
+        err = torch.ldexp(table[code] - scaled.abs(), ee - e).square().sum(-1, keepdim=True)
         code = code + 8 * (scaled < 0)
         if best is None:
             best = (err, code, ee)

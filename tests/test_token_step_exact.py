@@ -157,6 +157,24 @@ def test_w4_weight_loads_and_slices():
         assert getattr(part, name).data_ptr() == getattr(b, name)[7:].data_ptr()
 
 
+@pytest.mark.parametrize("octaves", [-110, -80, -60, 50, 70, 100, 120])
+def test_quantize_w4_at_any_size(octaves):
+    """Weights that are a power of two larger or smaller get the same codes, and
+    exponents that far apart: the better of two scales is found where the squares
+    of its errors are over or under fp32's range too."""
+    weight = torch.randn(64, 256, generator=gen(7)).clamp(-6, 6)
+    w, far = ops.quantize_w4(weight), ops.quantize_w4(weight * 2.0 ** octaves)
+    assert torch.equal(far.codes, w.codes) and torch.equal(far.exps.int(), w.exps.int() + octaves)
+
+
+def test_quantize_w4_refuses_what_32_bits_do_not_hold():
+    for bad in (1e39, -1e300):
+        weight = torch.zeros(2, 32, dtype=torch.float64)
+        weight[1, 5] = bad
+        with pytest.raises(ValueError):
+            ops.quantize_w4(weight)
+
+
 def test_w4_weight_leaves_a_loaded_state_alone():
     """A load, an assigning one too, writes nothing into what it was given."""
     for assign in (False, True):
