@@ -556,11 +556,11 @@ class T5ForConditionalGeneration(nn.Module):
         for blk in self.decoder.block:
             sa, ca, ff = blk.layer[0].SelfAttention, blk.layer[1].EncDecAttention, blk.layer[2].DenseReluDense
             linears += [sa.qkv, sa.o, ca.qkv, ca.o, ff.wi, ff.wo]
-        for lin in linears:
-            if not isinstance(lin.weight, ops.W4Weight):
-                w4 = ops.quantize_w4(lin.weight)
-                del lin.weight
-                lin.weight = w4
+        linears = [lin for lin in linears if not isinstance(lin.weight, ops.W4Weight)]
+        # all of them first: a weight that is refused leaves the model as it was
+        for lin, w4 in [(lin, ops.quantize_w4(lin.weight)) for lin in linears]:
+            del lin.weight
+            lin.weight = w4
         self._gen_graph = None   # it holds the old weights
         return self
 
