@@ -568,13 +568,14 @@ class T5ForConditionalGeneration(nn.Module):
     @torch.no_grad()
     def generate(self, input_ids=None, attention_mask=None, max_new_tokens: int = 128,
                  min_new_tokens: int = 0, eos_token_id=None, use_graph: bool | None = None,
-                 do_sample: bool = False, temperature: float = 1.0, top_k: int = 50,
-                 top_p: float = 1.0, min_p: float = 0.0,
+                 do_sample: bool = False, temperature: float | None = 1.0,
+                 top_k: int | None = 50, top_p: float | None = 1.0, min_p: float | None = 0.0,
                  generator: torch.Generator | None = None,
                  kv_cache_dtype: str | None = None, **_ignored):
         """Greedy decode, or with ``do_sample`` a token drawn at every step
-        after temperature, top-k, top-p and min-p (ops.sample_tokens; the
-        numbers come from ``generator``, or the device's default one).
+        after temperature, top-k, top-p and min-p (ops.sample_tokens; None
+        turns one off; the numbers come from ``generator``, or the device's
+        default one).
         ``kv_cache_dtype="fp8"`` holds the decoder's caches in 8 bits
         (ops.KVCache8).  On GPU with a fixed token budget
         (min_new_tokens == max_new_tokens) the whole decode loop is captured
@@ -590,8 +591,11 @@ class T5ForConditionalGeneration(nn.Module):
             raise ValueError(f"8-bit caches and 4-bit weights take a bf16 or fp16 model on a GPU, got {dt}")
         sampling = None
         if do_sample:
-            sampling = {"temperature": float(temperature), "top_k": int(top_k),
-                        "top_p": float(top_p), "min_p": float(min_p)}
+            def given(v, off):
+                return off if v is None else v
+
+            sampling = {"temperature": float(given(temperature, 1.0)), "top_k": int(given(top_k, 0)),
+                        "top_p": float(given(top_p, 1.0)), "min_p": float(given(min_p, 0.0))}
             ops.check_sampling(**sampling)
         if use_graph is None:
             use_graph = os.environ.get("MI355_GEN_GRAPH", "1") != "0"
