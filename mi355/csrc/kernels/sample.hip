@@ -53,7 +53,10 @@ constexpr int TABLE = 32;              // 8 bytes each: one for every pair of LD
 struct Opt {                             // a number for all rows, or one each
   const void* each;
   double all;
-  DEVINL double f(int row) const { return each ? (double)((const float*)each)[row] : all; }
+  bool wide;                             // fp64 ones
+  DEVINL double f(int row) const {
+    return !each ? all : wide ? ((const double*)each)[row] : (double)((const float*)each)[row];
+  }
   DEVINL int i(int row) const { return each ? ((const int*)each)[row] : (int)all; }
 };
 
@@ -767,13 +770,15 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
     if (!each.has_value() || !each->defined()) {
       VALUE_CHECK(all >= least && all <= most, "sampling: temperature and top_k are at least 0, "
                   "top_p and min_p from 0 to 1; got ", what, " = ", all);
-      return {nullptr, all};
+      return {nullptr, all, false};
     }
     VALUE_CHECK(each->dim() == 1 && each->size(0) == B && each->device() == logits.device(),
                 "sample_tokens: ", what, " must be a number or a (", B, ",) tensor on ",
                 logits.device(), ", got ", each->sizes(), " on ", each->device());
-    if (each->scalar_type() != type || !each->is_contiguous()) each = each->to(type).contiguous();
-    return {each->data_ptr(), all};
+    const bool wide = type == torch::kFloat && each->scalar_type() == torch::kDouble;
+    if ((!wide && each->scalar_type() != type) || !each->is_contiguous())
+      each = each->to(wide ? torch::kDouble : type).contiguous();
+    return {each->data_ptr(), all, wide};
   };
   const Opt ot = opt(temperatures, temperature, 0.0, 1.7e308, torch::kFloat, "temperature");
   const Opt ok = opt(top_ks, (double)std::min(top_k, V), 0.0, 1.7e308, torch::kInt, "top_k");

@@ -594,7 +594,7 @@ class T5ForConditionalGeneration(nn.Module):
             def given(v, off):
                 return off if v is None else v
 
-            sampling = {"temperature": float(given(temperature, 1.0)), "top_k": int(given(top_k, 0)),
+            sampling = {"temperature": float(given(temperature, 1.0)), "top_k": min(int(given(top_k, 0)), self.config.vocab_size),
                         "top_p": float(given(top_p, 1.0)), "min_p": float(given(min_p, 0.0))}
             ops.check_sampling(**sampling)
         if use_graph is None:
@@ -691,11 +691,10 @@ class T5ForConditionalGeneration(nn.Module):
         state = getattr(self, "_gen_graph", None)
         kpad = _kpad_from_mask(attention_mask)
         enc = self.encoder(input_ids=input_ids, kpad=kpad)
-        # What the capture bakes in: shapes, tokens, options, and where each
-        # weight lies.  Weights written in place are followed; ones that were
-        # cast, moved or replaced are somewhere else.
-        key = (b, input_ids.shape[1], max_new_tokens, str(dev), eos, kv8,
-               tuple(sampling.values()) if sampling is not None else None,
+        # What the capture bakes in: shapes, tokens, and where each weight lies.
+        # Weights written in place are followed; ones that were cast, moved or
+        # replaced are somewhere else.
+        key = (b, input_ids.shape[1], max_new_tokens, str(dev), eos, kv8, sampling is not None,
                cfg.decoder_start_token_id, cfg.pad_token_id, cfg.tie_word_embeddings,
                tuple((w.data_ptr(), w.dtype) for m in (self.decoder, self.lm_head)
                      for w in (*m.parameters(), *m.buffers())))
@@ -705,6 +704,11 @@ class T5ForConditionalGeneration(nn.Module):
             # build static buffers and capture the 128-step decode loop
             caches = self._decode_caches(enc, b, max_new_tokens, dev, dt, kv8)
             u_static = u.clone() if u is not None else None
+            # one value a row: other options are written here, not captured anew
+            options = None if sampling is None else {
+                name: torch.full((b,), value, device=dev,
+                                 dtype=torch.int32 if name == "top_k" else torch.float64)
+                for name, value in sampling.items()}
             enc_static = enc.clone()
             kpad_static = kpad.clone() if kpad is not None else None
             out_tokens = torch.zeros(b, max_new_tokens, device=dev, dtype=torch.long)
@@ -726,11 +730,11 @@ class T5ForConditionalGeneration(nn.Module):
                     logits = self._lm_logits(dec[:, -1])
                     if eos is not None:
                         logits[:, eos] = float("-inf")
-                    nxt = self._pick(logits, sampling, u_static[t] if u is not None else None)
+                    nxt = self._pick(logits, options, u_static[t] if u is not None else None)
                     out_tokens[:, t] = nxt
                     tok = nxt.unsqueeze(1)
             state = {"key": key, "graph": g, "enc": enc_static, "kpad": kpad_static,
-                     "caches": caches, "out": out_tokens, "u": u_static,
+                     "caches": caches, "out": out_tokens, "u": u_static, "options": options,
                      "bias": bias_static}
             self._gen_graph = state
         # refresh the static inputs, reset self-cache lengths, replay
@@ -740,6 +744,8 @@ class T5ForConditionalGeneration(nn.Module):
             state["kpad"].copy_(kpad)
         if u is not None:
             state["u"].copy_(u)
+            for name, value in sampling.items():
+                state["options"][name].fill_(value)
         if kv8:
             self._fill_cross_kv8(state["caches"], enc, b)
         else:

@@ -31,7 +31,8 @@ def _per_row(v, what: str, rows: int, device, dtype):
     if v.shape != (rows,) or v.device != device:
         raise ValueError(f"{what} must be a number or a ({rows},) tensor on {device}, "
                          f"got {tuple(v.shape)} on {v.device}")
-    return (v if v.dtype == dtype else v.to(dtype)).contiguous(), 0
+    wide = dtype == torch.float32 and v.dtype == torch.float64
+    return (v if v.dtype == dtype or wide else v.to(dtype)).contiguous(), 0
 
 
 # --------------------------------------------------------------------------- #
@@ -281,8 +282,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     those the ones with w >= ``min_p``; the token is the lowest index whose
     running sum of kept weights, in index order, is over u times their sum.
     Weights and sums are in 64 bits.  temperature 0 takes the first of the
-    order.  Options are numbers, or a value for each row: float32 (B,) tensors
-    (int32 for top_k); values from tensors that are out of range count as the
+    order.  Options are numbers, or a value for each row: float32 or float64
+    (B,) tensors (int32 for top_k); values from tensors that are out of range count as the
     nearest in range.  NaN counts as -inf; a row with nothing above -inf gives
     ``empty_token``.  Weights under 2^-45 of the largest count as 0.
     Returns int64 (B,).

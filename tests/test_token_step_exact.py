@@ -8,7 +8,8 @@ import torch
 
 from mi355 import ops
 
-from test_token_step import BF16, DEVICES, FP16, FP32, Plain8, gen, gpu, w4_values  # noqa: F401
+from test_token_step import (BF16, DEVICES, FP16, FP32, Plain8, gen, gpu, sample_by_definition,  # noqa: F401
+                             uniform, w4_values)
 
 
 # --------------------------------------------------------------------------- #
@@ -246,3 +247,26 @@ def test_kv8_append_one_grows_at_every_offset(device, dtype, d):
     plain.append(new[0], new[1], start)
     plain.same(cache)
     assert bool((cache.k_scale > before[0]).all()) and bool((cache.v_scale > before[1]).all())
+
+
+# --------------------------------------------------------------------------- #
+# sampling                                                                    #
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("device", DEVICES)
+def test_sample_tokens_options_of_64_bits(device):
+    """A row's options in 64 bits are those numbers, as one number for all rows
+    is: 0.3 of ten equal weights is three of them, and what fp32 makes of it four."""
+    logits = torch.zeros(4, 10, device=device)
+    u = torch.full((4,), 0.9999, device=device)
+    p = torch.full((4,), 0.3, dtype=torch.float64, device=device)
+    assert ops.sample_tokens(logits, u, top_p=0.3).tolist() == [2] * 4
+    assert ops.sample_tokens(logits, u, top_p=p).tolist() == [2] * 4
+    assert ops.sample_tokens(logits, u, top_p=p.float()).tolist() == [3] * 4
+    g = gen(31)
+    logits = (torch.randn(40, 3001, generator=g) * 3).to(device)
+    u = uniform(40, 32, device, torch.float64)
+    r = torch.rand(3, 40, generator=g, dtype=torch.float64).to(device)
+    opt = dict(temperature=0.3 + r[0], top_k=0, top_p=1 - 0.3 * r[1], min_p=0.05 * r[2])
+    assert ops.sample_tokens(logits, u, **opt).tolist() == sample_by_definition(logits, u, **opt)
+    rows = dict(opt, temperature=opt["temperature"].float(), top_p=opt["top_p"][:1].expand(40))
+    assert ops.sample_tokens(logits, u, **rows).tolist() == sample_by_definition(logits, u, **rows)
