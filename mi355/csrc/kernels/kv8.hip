@@ -16,6 +16,8 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <limits>
+
 #include "../common.h"
 
 namespace {
@@ -688,9 +690,11 @@ Cache check_cache(const torch::Tensor& k, const torch::Tensor& v, const torch::T
 PerSeq per_seq(c10::optional<torch::Tensor>& each, long all, const Cache& c, const char* what) {
   if (each.has_value() && each->defined()) {
     VALUE_CHECK(each->dim() == 1 && each->size(0) == c.B && each->device() == c.k.device() &&
-                    !each->is_floating_point(),
+                    c10::isIntegralType(each->scalar_type(), /*includeBool=*/false),
                 "kv8: ", what, " must be a number or an int32 (", c.B, ",) tensor on ",
                 c.k.device(), ", got ", each->sizes(), " on ", each->device());
+    if (each->scalar_type() == torch::kLong)        // past every capacity, or under 0, either way
+      each = each->clamp(std::numeric_limits<int>::min(), std::numeric_limits<int>::max());
     if (each->scalar_type() != torch::kInt || !each->is_contiguous())
       each = each->to(torch::kInt).contiguous();
     return {each->data_ptr<int>(), 0};

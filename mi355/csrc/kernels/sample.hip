@@ -776,6 +776,9 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
                 "sample_tokens: ", what, " must be a number or a (", B, ",) tensor on ",
                 logits.device(), ", got ", each->sizes(), " on ", each->device());
     const bool wide = type == torch::kFloat && each->scalar_type() == torch::kDouble;
+    // a top-k of another type: over MAX_V, where it keeps all, its size is not needed
+    if (type == torch::kInt && each->scalar_type() != type)
+      each = each->to(torch::kDouble).nan_to_num(0.0).clamp(-1.0, 2.0 * MAX_V);
     if ((!wide && each->scalar_type() != type) || !each->is_contiguous())
       each = each->to(wide ? torch::kDouble : type).contiguous();
     return {each->data_ptr(), all, wide};

@@ -28,9 +28,13 @@ def _per_row(v, what: str, rows: int, device, dtype):
     """(tensor or None, number): one value for every row, or a number for all."""
     if not torch.is_tensor(v):
         return None, v
+    if dtype == torch.int32 and what != "top_k" and (v.is_floating_point() or v.is_complex() or v.dtype == torch.bool):
+        raise ValueError(f"{what} must be whole numbers, got {v.dtype}")
     if v.shape != (rows,) or v.device != device:
         raise ValueError(f"{what} must be a number or a ({rows},) tensor on {device}, "
                          f"got {tuple(v.shape)} on {v.device}")
+    if dtype == torch.int32 and v.dtype != dtype:   # no number becomes another one
+        v = v.double().nan_to_num(0.0).clamp(-2.0 ** 31, 2.0 ** 31 - 1)
     wide = dtype == torch.float32 and v.dtype == torch.float64
     return (v if v.dtype == dtype or wide else v.to(dtype)).contiguous(), 0
 

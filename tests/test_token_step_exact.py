@@ -270,3 +270,48 @@ def test_sample_tokens_options_of_64_bits(device):
     assert ops.sample_tokens(logits, u, **opt).tolist() == sample_by_definition(logits, u, **opt)
     rows = dict(opt, temperature=opt["temperature"].float(), top_p=opt["top_p"][:1].expand(40))
     assert ops.sample_tokens(logits, u, **rows).tolist() == sample_by_definition(logits, u, **rows)
+
+
+# --------------------------------------------------------------------------- #
+# whole numbers of another type                                               #
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("device", DEVICES)
+def test_whole_numbers_of_64_bits_keep_their_value(device):
+    """Positions, counts, lengths and top-k of int64 mean what they say: none is
+    taken modulo 2^32."""
+    def whole(*v):
+        return torch.tensor(v, dtype=torch.int64, device=device)
+
+    b, h, d, s = 5, 2, 64, 70
+    k, v = (torch.randn(2, b, h, s, d, generator=gen(41)).to(device, BF16))
+    start, counts = whole(2 ** 32, -2 ** 32 - 1, 2 ** 33 + 5, 3, 60), whole(4, 4, 4, 2 ** 32 + 1, -2 ** 33)
+    cache, plain = ops.KVCache8(b, h, 256, d, device=device), Plain8(b, h, 256, d)
+    ops.kv8_append(cache, k, v, start, counts)
+    plain.append(k, v, start, counts)
+    plain.same(cache)
+    one, plain1 = ops.KVCache8(b, h, 256, d, device=device), Plain8(b, h, 256, d)
+    ops.kv8_append(one, k[:, :, :1], v[:, :, :1], start)
+    plain1.append(k[:, :, :1], v[:, :, :1], start)
+    plain1.same(one)
+    q = torch.randn(b, h, 1, d, generator=gen(42)).to(device, BF16)
+    ops.kv8_append(cache, k, v, 0)
+    got = ops.decode_attention_kv8(q, cache, whole(2 ** 32, 2 ** 40 + 3, -2 ** 32 + 9, 3, 70), max_len=70)
+    want = ops.decode_attention_kv8(q, cache, torch.tensor([70, 70, 0, 3, 70], dtype=torch.int32, device=device), max_len=70)
+    assert torch.equal(got, want)
+    logits, u = torch.randn(5, 1000, generator=gen(43)).to(device), torch.full((5,), 0.97, device=device)
+    every = ops.sample_tokens(logits, u, temperature=3.0)
+    assert torch.equal(ops.sample_tokens(logits, u, temperature=3.0, top_k=whole(2 ** 32 + 1, 2 ** 62, 0, -2 ** 32 + 1, 10 ** 6)), every)
+    for top_k in (torch.tensor([1e12, 2.0 ** 31, math.inf, 0.0, -1e12], device=device), whole(0, 0, 0, 0, 0).to(torch.uint8)):
+        assert torch.equal(ops.sample_tokens(logits, u, temperature=3.0, top_k=top_k), every)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, FP16, torch.float64, torch.bool])
+def test_positions_that_are_no_whole_numbers_are_refused(device, dtype):
+    cache = ops.KVCache8(2, 3, 100, 64, device=device)
+    k = torch.randn(2, 3, 4, 64, generator=gen(44)).to(device, BF16)
+    at = torch.ones(2, dtype=dtype, device=device)
+    for bad in (lambda: ops.kv8_append(cache, k, k, at), lambda: ops.kv8_append(cache, k, k, 0, counts=at),
+                lambda: ops.decode_attention_kv8(k[:, :, :1], cache, at)):
+        with pytest.raises(ValueError):
+            bad()
