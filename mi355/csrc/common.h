@@ -117,6 +117,9 @@ DEVINL float hash_u01(long long seed, long long idx) {
     if (!(cond)) throw pybind11::value_error(c10::str(__VA_ARGS__)); \
   } while (0)
 
+// A launch has fewer than 2^32 threads in a dimension.
+constexpr bool fits_a_launch(long workgroups, long threads) { return workgroups < (1L << 32) / threads; }
+
 // Operators without a backward pass refuse inputs that ask for a gradient.
 #define NO_GRAD_CHECK(t, what)                                     \
   TORCH_CHECK(!(t).requires_grad() || !at::GradMode::is_enabled(), \

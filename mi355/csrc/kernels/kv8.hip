@@ -736,10 +736,11 @@ void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tenso
               " do not fit a cache of ", c.NB * BLK);
   const PerSeq ct = per_seq(counts, S, c, "counts");
   if (S == 0 || c.B * c.H == 0) return;
+  const long NW = (S + BLK - 2) / BLK + 1;
+  VALUE_CHECK(S < (1L << 30) && fits_a_launch(S == 1 ? (c.B * c.H + 3) / 4 : c.B * c.H * NW, 256),
+              "kv8_append: too many tokens at once: ", k.sizes());
   k = rows16(k);
   v = rows16(v);
-  const long NW = (S + BLK - 2) / BLK + 1;
-  VALUE_CHECK(c.B * c.H * NW < (1L << 31), "kv8_append: too many tokens at once");
   auto stream = at::hip::getCurrentHIPStream().stream();
   const Str3 kst{k.stride(0), k.stride(1), k.stride(2)}, vst{v.stride(0), v.stride(1), v.stride(2)};
 #define APPEND(T, DD)                                                                            \
@@ -830,7 +831,9 @@ torch::Tensor kv8_attn(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torc
   torch::Tensor part;
   if (nsplit > 1) part = torch::empty({c.B * Hq * nsplit * (c.D + 2)}, ks.options());
   auto stream = at::hip::getCurrentHIPStream().stream();
-  const dim3 grid((c.B * c.H + 4 / a.share - 1) / (4 / a.share), nsplit, nz);
+  const long groups = (c.B * c.H + 4 / a.share - 1) / (4 / a.share);
+  VALUE_CHECK(fits_a_launch(groups, 256), "decode_attention_kv8: too many heads: ", kc.sizes());
+  const dim3 grid(groups, nsplit, nz);
   auto run = [&](auto kernel, auto* type) {
     using T = std::remove_pointer_t<decltype(type)>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const T*)q.data_ptr(),

@@ -758,7 +758,7 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u,
   VALUE_CHECK(logits.dim() == 2 && logits.is_cuda() && logits.size(1) >= 1 && logits.size(1) <= MAX_V,
               "sample_tokens: logits (B, V) with V from 1 to ", MAX_V, ", got ", logits.sizes());
   const long B = logits.size(0), V = logits.size(1);
-  VALUE_CHECK(B < (1L << 31), "sample_tokens: too many rows");
+  VALUE_CHECK(fits_a_launch(B, THREADS), "sample_tokens: too many rows: ", B);
   VALUE_CHECK(u.dim() == 1 && u.size(0) == B && u.device() == logits.device() &&
                   (u.scalar_type() == torch::kFloat || u.scalar_type() == torch::kDouble),
               "sample_tokens: u must be fp32 or fp64 (", B, ",) on ", logits.device(), ", got ",

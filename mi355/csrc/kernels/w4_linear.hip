@@ -484,13 +484,15 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
   VALUE_CHECK(x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kHalf,
               "linear_w4 takes bf16 or fp16 on a GPU, got ", x.scalar_type());
   c10::DeviceGuard guard(x.device());
+  const long M = x.numel() / K;
+  // tiles of 32 rows take 256 threads and of 64 rows 512; a grid's second dimension, of
+  // tiles of 32 outputs and more, is 16 bits wide
+  VALUE_CHECK(fits_a_launch((M + 31) / 32, 256) && N < 65535L * 32 && K < (1L << 30),
+              "linear_w4: too large: ", M, " rows of ", K, " by ", N);
   auto sizes = x.sizes().vec();
   sizes.back() = N;
   auto y = at::empty(sizes, x.options().memory_format(at::MemoryFormat::Contiguous));
   if (x.dim() != 2) x = x.reshape({-1, K});
-  const long M = x.size(0);
-  // a grid's second dimension is 16 bits wide: blocks of 16 rows, of 32 outputs
-  VALUE_CHECK(M < (1L << 31) - 256 && N < 65535L * 32 && K < (1L << 30), "linear_w4: too large");
   if (M == 0 || N == 0) return y;
   // rows of x are read 16 bytes at a time
   if (x.stride(1) != 1 || (M > 1 && x.stride(0) % 8 != 0) ||

@@ -315,3 +315,28 @@ def test_positions_that_are_no_whole_numbers_are_refused(device, dtype):
                 lambda: ops.decode_attention_kv8(k[:, :, :1], cache, at)):
         with pytest.raises(ValueError):
             bad()
+
+
+# --------------------------------------------------------------------------- #
+# sizes over what a launch can have                                           #
+# --------------------------------------------------------------------------- #
+@gpu
+def test_more_workgroups_than_a_launch_has_are_refused():
+    """A launch has fewer than 2^32 threads: as many rows, heads and tokens as
+    would take more are refused before anything runs."""
+    def wide(*shape, dtype=BF16):
+        return torch.zeros([1] * len(shape), dtype=dtype, device="cuda").expand(shape)
+
+    n = 1 << 22                                          # rows of 1024 threads
+    with pytest.raises(ValueError):
+        ops.sample_tokens(wide(n, 8), wide(n, dtype=FP32))
+    n = 1 << 29                                          # 32 rows for 256 threads
+    w = ops.quantize_w4(torch.zeros(1, 32, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.linear_w4(torch.zeros(32, dtype=BF16, device="cuda").expand(n, 32), w)
+    start = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for heads, tokens in ((1 << 26, 1), (1 << 23, 2)):   # four heads, and half a head, for 256 threads
+        cache = ops.KVCache8(1, heads, 0, 32, device="cuda")
+        k = torch.zeros(32, dtype=BF16, device="cuda").expand(1, heads, tokens, 32)
+        with pytest.raises(ValueError):
+            ops.kv8_append(cache, k, k, start)
