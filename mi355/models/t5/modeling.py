@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import math
 import os
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -24,6 +25,9 @@ from ... import ops
 from .configuration import T5Config, t5_config
 
 NEG_INF = -1e9
+# held while a captured decode loop is made, or filled and launched: its buffers
+# are one set for all calls (not on the model, which has to stay copyable)
+_GRAPH_LOCK = threading.Lock()
 
 
 class T5LayerNorm(nn.Module):
@@ -604,8 +608,9 @@ class T5ForConditionalGeneration(nn.Module):
             # drawn before the attempt, so that the eager fallback has them too
             u = self._uniforms(sampling, max_new_tokens, input_ids, generator)
             try:
-                return self._generate_graphed(input_ids, attention_mask, max_new_tokens,
-                                              eos_token_id, sampling, u, kv8)
+                with _GRAPH_LOCK:
+                    return self._generate_graphed(input_ids, attention_mask, max_new_tokens,
+                                                  eos_token_id, sampling, u, kv8)
             except Exception as e:
                 if not getattr(self, "_gen_graph_warned", False):
                     self._gen_graph_warned = True
@@ -735,8 +740,11 @@ class T5ForConditionalGeneration(nn.Module):
                     tok = nxt.unsqueeze(1)
             state = {"key": key, "graph": g, "enc": enc_static, "kpad": kpad_static,
                      "caches": caches, "out": out_tokens, "u": u_static, "options": options,
-                     "bias": bias_static}
+                     "bias": bias_static, "done": torch.cuda.Event()}
             self._gen_graph = state
+        else:
+            # the last call's replay, maybe on another stream, has read its inputs
+            torch.cuda.current_stream(dev).wait_event(state["done"])
         # refresh the static inputs, reset self-cache lengths, replay
         state["enc"].copy_(enc)
         state["bias"].copy_(full_bias)
@@ -755,7 +763,9 @@ class T5ForConditionalGeneration(nn.Module):
                 state["caches"][i]["cross"]["v"].copy_(kv_pairs[i][1])
                 state["caches"][i]["self"]["len"] = 0
         state["graph"].replay()
-        return state["out"].clone()
+        out = state["out"].clone()
+        state["done"].record(torch.cuda.current_stream(dev))
+        return out
 
     @torch.no_grad()
     def _generate_eager(self, input_ids=None, attention_mask=None, max_new_tokens: int = 128,

@@ -1,6 +1,7 @@
 """The captured decode loop of generate() follows what became of the model since
 the capture."""
 import copy
+import threading
 
 import pytest
 import torch
@@ -90,3 +91,41 @@ def test_captured_loop_follows_the_position_bias(options):
         out = both(m, **options)
         assert torch.equal(*out) and not torch.equal(out[0], before)
     assert m._gen_graph is state
+
+
+@gpu
+@pytest.mark.parametrize("options", [dict(), dict(kv_cache_dtype="fp8", do_sample=True, temperature=2.0)])
+@pytest.mark.parametrize("threads", [False, True])
+def test_captured_loop_on_streams_and_threads(options, threads):
+    """Calls on streams of their own, and from threads, without a
+    synchronization between: each gives the tokens of its own prompt."""
+    m = model("cuda")
+    ids = torch.randint(2, 512, (6, 3, 12), generator=torch.Generator().manual_seed(8)).cuda()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+
+    def call(i, use_graph):
+        return m.generate(input_ids=ids[i], max_new_tokens=40, min_new_tokens=40, use_graph=use_graph,
+                          generator=seeded("cuda", i), **options)
+
+    want = [call(i, False) for i in range(6)]
+    call(0, True)
+    torch.cuda.synchronize()
+    got = [[] for _ in range(6)]
+
+    def run(i):
+        with torch.cuda.stream(streams[i % 3]):
+            for _ in range(4):
+                got[i].append(call(i, True))
+
+    if threads:
+        workers = [threading.Thread(target=run, args=(i,)) for i in range(6)]
+        for w in workers:
+            w.start()
+        for w in workers:
+            w.join()
+    else:
+        for i in range(6):
+            run(i)
+    torch.cuda.synchronize()
+    assert all(len(g) == 4 and torch.equal(x, w) for g, w in zip(got, want) for x in g)
+    assert not getattr(m, "_gen_graph_warned", False)
