@@ -155,9 +155,11 @@ DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, const T* 
 // ---------------------------------------------------------------------------
 // Up to 16 rows, x straight from the caches: one wave owns 16*NT outputs and
 // every WAVES-th 128-wide piece of K, the next piece's weights and x on their
-// way while this one is multiplied.  NT tiles of outputs share a wave's x: 16
-// rows by 10240 x 2048 take 8.1 us with four of them, 10.6 with one; 16 rows by
-// 2304 x 768, too few outputs for that, 3.8 and 3.1 us.
+// way while this one is multiplied.  NT tiles of outputs share a wave's x: as few
+// as leave at most 256 workgroups, one a CU, and four beyond.  A call with 16 rows
+// and K = 2048 takes with one, two and four tiles 5.5, 5.9 and 7.9 us for 4096
+// outputs; 7.6, 5.9 and 7.9 for 4608; 7.8, 6.0 and 7.9 for 8192; 10.3, 9.5 and 8.0
+// for 8704; 19.4, 14.0 and 14.1 for 20480; 27.1, 17.9 and 14.3 for 32128.
 // ---------------------------------------------------------------------------
 template <typename T, int NT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
@@ -228,9 +230,15 @@ __host__ __device__ constexpr int lds_row(int K) { return (K + 255) / 256 * 256 
 // beside its weights: of the 64 lanes that the matrix instruction has for x only
 // M in 16 hold a row (the others repeat the last; their sums are not stored),
 // and fetching those from the caches takes as many memory instructions as the
-// weights.  U pieces of 128 lie next to each other.  One row by 20480 x 4096:
-// 12.7 us (3.5 TB/s of weights) here with 4 waves of two pieces, 13.5 with 8 of
-// one, 17 with x from the caches; 16 rows by 10240 x 2048 11 against 8.1.
+// weights.  One row by 20480 x 4096: 12.0 us (3.7 TB/s), 17 with x from the caches;
+// by 10240 x 2048 a call with 4 rows takes 6.2 us, 7.2 with x from the caches, with
+// 8 rows 7.3 and 7.5, with 12 rows 10.2 and 7.7.
+// U pieces of 128 lie next to each other.  Eight waves of one piece, but four of
+// two for many outputs and a K under 1024, of which either takes all at once and
+// more, smaller workgroups fill the CUs better: one row by 32128 x 768 5.4 us (6.0
+// with eight waves), 8 rows 6.9 (7.2), one by 50257 x 768 7.7 (8.0); by 18432 x 768
+// 5.5 and 5.4; by 32128 x 1024 6.9 and 6.8, x 2048 10.7 and 10.4, with 8 rows x 2304
+// 19.6 and 16.3.
 template <typename T, int NT, int U, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64)
 w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
@@ -315,15 +323,22 @@ w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
 // of a lane group as a plane of its own, rows 80 bytes apart and planes a
 // multiple of 256: sixteen rows at one k are in different banks, in whichever
 // lane groups the hardware takes them.
-// Tiles of 128 x 128 once there are 128 of them for the 256 CUs, else of
-// 64 x 64 once there are 128, else of 32 x 32: 256 rows by 10240 x 2048 take
-// 25, 34 and 53 us, by 4096 x 768 11, 6.6 and 9.5 us, by 768 x 2048 23, 12 and
-// 7.8 us (the library on 16-bit weights: 23, 6.8 and 8.4 us).  Four waves of 64 x
-// 64 read half as much LDS as eight of 64 x 32, but 30 us, one for each SIMD, is
-// more than 25.  Where there are
-// few tiles and a long K, tiles of 64 x 64 share K, in runs of 512 and more,
-// and a second kernel adds their fp32 sums: 64 rows by 4096 x 10240 34 -> 20 us,
-// 128 by 2048 x 5120 18 -> 14; 64 by 1024 x 2816, too short, 9.0 and 8.9.
+// 256 rows by 10240 x 2048 take 25, 34 and 53 us in tiles of 128 x 128, 64 x 64 and
+// 32 x 32, by 4096 x 768 11, 6.6 and 9.5 us, by 768 x 2048 23, 12 and 8.9 us (the
+// library on 16-bit weights: 23, 6.8 and 8.4 us).  Which it is follows from rounds
+// of workgroups on the 256 CUs; of each border both sides, in us a call:
+//  - 128 x 128 for over 64 rows and over 512 tiles of 64 x 64.  256 rows by 8448 x
+//    2048 25.6 (64 x 64: 34.8), by 8192 x 2048 24.6 (23.9); 96 rows by 32128 x 768
+//    12.9 (18.1), 64 rows by 40000 x 768 21.9 (15.8).
+//  - 64 x 64 for over 32 rows and over 128 tiles.  256 rows by 2560 x 2048 13.1 (32 x
+//    32: 17.4), by 2048 x 2048 13.0 (12.5); 33 rows by 10240 x 2048 13.6 (18.0),
+//    32 rows 13.4 (12.5).
+//  - Up to 128 tiles of 64 x 64 and K from 4096: they share K, in runs of 512 and
+//    more, and a second kernel adds their fp32 sums in order.  64 rows by 4096 x
+//    10240 24.2 (32 x 32: 42.5), 256 by 2048 x 4096 18.4 (21.5); 192 by 4096 x 4096,
+//    192 tiles, 29.9 (64 x 64: 24.6); 64 by 4096 x 2816 10.9 (10.5).
+// Four waves of 64 x 64 read half as much LDS as eight of 64 x 32, but 30 us, one
+// for each SIMD, is more than 25.
 // ---------------------------------------------------------------------------
 template <typename T, int MT, int NT, int WN>
 __global__ void __launch_bounds__(128 * WN)
@@ -523,18 +538,20 @@ torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps
     const auto tiles = [&](long t) { return dim3(up(M, t), up(N, t)); };
     const auto count = [](dim3 d) { return (long)d.x * d.y; };
     const long copy = M * lds_row(K) * 2;           // x in LDS
+    // What bounds a launch is rounds of workgroups on the 256 CUs; the borders, with
+    // both sides of each, are at the kernels.
     if (M <= 8 && copy <= 56 * 1024) {
-      if (M <= 2 && N >= 16384) launch(w4_lds_rows<T, 1, 2, 4>, dim3(up(N, 16)), 256, copy);
+      if (N >= 20480 && K < 1024) launch(w4_lds_rows<T, 1, 2, 4>, dim3(up(N, 16)), 256, copy);
       else launch(w4_lds_rows<T, 1, 1, 8>, dim3(up(N, 16)), 512, copy);
     } else if (M <= 16) {
-      if (N < 8192) launch(w4_few_rows<T, 1, 8>, dim3(up(N, 16)), 512, 0);
-      else if (M <= 8) launch(w4_few_rows<T, 2, 8>, dim3(up(N, 32)), 512, 0);
+      if (N <= 4096) launch(w4_few_rows<T, 1, 8>, dim3(up(N, 16)), 512, 0);
+      else if (N <= 8192) launch(w4_few_rows<T, 2, 8>, dim3(up(N, 32)), 512, 0);
       else launch(w4_few_rows<T, 4, 8>, dim3(up(N, 64)), 512, 0);
-    } else if (count(tiles(128)) >= 128) {
+    } else if (M > 64 && count(tiles(64)) > 512) {
       many(w4_many_rows<T, 4, 2, 4>, tiles(128), 512, 1);
-    } else if (K >= 4096 && count(tiles(64)) < 256) {
+    } else if (K >= 4096 && count(tiles(64)) <= 128) {
       many(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, std::min(up(256, count(tiles(64))), K / 512));
-    } else if (count(tiles(64)) >= 128) {
+    } else if (M > 32 && count(tiles(64)) > 128) {
       many(w4_many_rows<T, 2, 1, 4>, tiles(64), 512, 1);
     } else {
       many(w4_many_rows<T, 1, 1, 2>, tiles(32), 256, 1);

@@ -15,11 +15,12 @@ from test_token_step import (BF16, DEVICES, FP16, FP32, Plain8, gen, gpu, sample
 # --------------------------------------------------------------------------- #
 # 4-bit weights                                                               #
 # --------------------------------------------------------------------------- #
-# every kernel, of few rows and of many: x in LDS (of both forms), x from the
-# caches (of one, two and four tiles), tiles of 128, of 64 with and without
+# every kernel, of few rows and of many: x in LDS (of eight waves, of four), x from
+# the caches (of one, two and four tiles), tiles of 128, of 64 with and without
 # shared K, of 32
 W4_SHAPES = [(1, 40, 96), (2, 24, 512), (8, 40, 416), (2, 16390, 96), (8, 40, 4640), (12, 40, 160), (8, 8200, 4640),
-             (12, 8210, 160), (130, 8200, 96), (70, 70, 4128), (129, 2700, 128), (40, 40, 416)]
+             (12, 8210, 160), (130, 8200, 96), (70, 70, 4128), (129, 2700, 128), (40, 40, 416),
+             (3, 20490, 96), (12, 4200, 160), (7, 4100, 4640), (130, 11100, 96), (20, 4100, 4128)]
 SPANS = [0, 20, 22, 23, 24, 30, 35, 36, 37, 38, 50, 60, 99, 101, 134]     # octaves between a row's scales
 
 
@@ -340,3 +341,20 @@ def test_more_workgroups_than_a_launch_has_are_refused():
         k = torch.zeros(32, dtype=BF16, device="cuda").expand(1, heads, tokens, 32)
         with pytest.raises(ValueError):
             ops.kv8_append(cache, k, k, start)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", [(1, 20480, 992), (8, 20479, 736), (1, 20480, 1024), (9, 4096, 288), (16, 4097, 288),
+                                   (13, 8192, 288), (13, 8193, 288), (65, 16384, 96), (65, 16385, 96), (64, 32800, 64),
+                                   (33, 8256, 96), (33, 8192, 96), (32, 8256, 96), (128, 4096, 4096), (129, 2752, 4096),
+                                   (17, 8192, 4096)])
+def test_linear_w4_where_one_kernel_follows_another(device, dtype, m, n, k):
+    """Sizes at which another kernel takes over."""
+    if device == "cpu" and m * n * k > 10 ** 8:
+        n = n % 1021
+    codes = torch.randint(0, 256, (n, k // 2), generator=gen(m + n), dtype=torch.uint8)
+    exps = torch.randint(117, 124, (n, k // 32), generator=gen(k), dtype=torch.uint8)
+    w = ops.W4Weight(codes.to(device), exps.to(device))
+    x = torch.randn(m, k, generator=gen(51)).to(device, dtype)
+    check_group_sums(x, w, ops.linear_w4(x, w))
