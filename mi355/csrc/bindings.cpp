@@ -80,6 +80,7 @@ std::vector<torch::Tensor> attn_bwd_v3(torch::Tensor dout, torch::Tensor q, torc
                                        c10::optional<torch::Tensor> packed);
 torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps,
                         torch::Tensor row_exp);
+torch::Tensor w4_row_exp(torch::Tensor codes, torch::Tensor exps);
 void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tensor vc,
                 torch::Tensor ks, torch::Tensor vs, c10::optional<torch::Tensor> starts, long start,
                 c10::optional<torch::Tensor> counts);
@@ -136,6 +137,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kpad"), py::arg("causal"), py::arg("need_dbias"),
         py::arg("p_drop"), py::arg("seed"), py::arg("packed") = c10::nullopt);
   m.def("w4_linear", &w4_linear);
+  m.def("w4_row_exp", &w4_row_exp);
   m.def("kv8_append", &kv8_append);
   m.def("kv8_attn", &kv8_attn);
   m.def("sample_tokens", &sample_tokens);

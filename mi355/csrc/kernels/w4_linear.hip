@@ -89,6 +89,36 @@ struct Args {
 
 constexpr int FAR = 255;                // the row exponent of rows without one scale for all
 
+constexpr int SPAN = 26;                // octaves that a row may span otherwise
+
+// Each row's exponent, a wave a row and a lane a group: the largest of groups that
+// hold more than zeros, or FAR.  Once for a weight; bound by reading its codes.
+__global__ void __launch_bounds__(256)
+w4_row_exp_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exps,
+                  unsigned char* __restrict__ row_exp, int N, int groups) {
+  const int lane = threadIdx.x & 63;
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= N) return;
+  int most = 0, least = 255, no_scale = 0;
+  for (int g = lane; g < groups; g += 64) {
+    const long at = (long)n * groups + g;
+    u32x4 c;
+    __builtin_memcpy(&c, codes + 16 * at, 16);      // of any alignment
+    const int e = exps[at];
+    const bool there = ((c[0] | c[1] | c[2] | c[3]) & 0x77777777u) != 0;
+    most = max(most, there ? e : 0);
+    least = min(least, there ? e : 255);
+    no_scale |= e == 255;
+  }
+#pragma unroll
+  for (int by = 32; by > 0; by >>= 1) {
+    most = max(most, __shfl_xor(most, by));
+    least = min(least, __shfl_xor(least, by));
+    no_scale |= __shfl_xor(no_scale, by);
+  }
+  if (lane == 0) row_exp[n] = no_scale || most - least > SPAN ? FAR : most;
+}
+
 // One output of such a row: a sum in fp32 for each group, its scale, their sum.
 template <typename T> DEVINL float far_output(const T* x, const Args& a, int m, int n) {
   const unsigned char* codes = a.codes + (long)n * (a.K >> 1);
@@ -479,6 +509,26 @@ w4_add_parts(const T* __restrict__ x, const float* __restrict__ part, T* __restr
 }
 
 }  // namespace
+
+torch::Tensor w4_row_exp(torch::Tensor codes, torch::Tensor exps) {
+  VALUE_CHECK(codes.dim() == 2 && exps.dim() == 2 && codes.size(0) == exps.size(0) &&
+                  codes.size(1) == 16 * exps.size(1) && exps.size(1) < (1L << 25) &&
+                  fits_a_launch((codes.size(0) + 3) / 4, 256),
+              "w4_row_exp: codes (N,K/2) and exponents (N,K/32), got ", codes.sizes(), " and ", exps.sizes());
+  for (const auto* t : {&codes, &exps})
+    VALUE_CHECK(t->scalar_type() == torch::kByte && t->is_contiguous() && t->is_cuda() &&
+                    t->device() == codes.device(),
+                "w4_row_exp: contiguous uint8 tensors of one GPU");
+  c10::DeviceGuard guard(codes.device());
+  auto row_exp = at::empty({codes.size(0)}, exps.options());
+  if (codes.size(0) == 0) return row_exp;
+  hipLaunchKernelGGL(w4_row_exp_kernel, dim3((codes.size(0) + 3) / 4), dim3(256), 0,
+                     at::hip::getCurrentHIPStream().stream(), codes.data_ptr<unsigned char>(),
+                     exps.data_ptr<unsigned char>(), row_exp.data_ptr<unsigned char>(),
+                     (int)codes.size(0), (int)exps.size(1));
+  HIP_CHECK_KERNEL();
+  return row_exp;
+}
 
 torch::Tensor w4_linear(torch::Tensor x, torch::Tensor codes, torch::Tensor exps,
                         torch::Tensor row_exp) {

@@ -67,12 +67,16 @@ class W4Weight(torch.nn.Module):
             raise ValueError(f"codes on {codes.device}, exponents on {exps.device}")
         self.register_buffer("codes", codes.contiguous())
         self.register_buffer("exps", exps.contiguous())
-        self.register_buffer("row_exp", torch_ref.w4_row_exp(codes, exps))
+        self.register_buffer("row_exp", self._row_exp())
+
+    def _row_exp(self) -> torch.Tensor:
+        make = _load_ext().w4_row_exp if _use_hip(self.codes) else torch_ref.w4_row_exp
+        return make(self.codes.contiguous(), self.exps.contiguous())
 
     def _load_from_state_dict(self, *args, **kwargs):
         row_exp = self.row_exp
         super()._load_from_state_dict(*args, **kwargs)
-        fresh = torch_ref.w4_row_exp(self.codes, self.exps)
+        fresh = self._row_exp()
         if self.row_exp is row_exp:
             row_exp.copy_(fresh)
         else:                                   # the caller's tensor, of an assigning load

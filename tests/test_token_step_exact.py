@@ -177,6 +177,33 @@ def test_quantize_w4_refuses_what_32_bits_do_not_hold():
             ops.quantize_w4(weight)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n,k", [(1, 32), (5, 64), (300, 96), (67, 2048), (9, 4640), (130, 4128)])
+def test_w4_row_exponents(device, n, k):
+    """Each row's largest exponent of groups with codes other than 0 and -0; 255
+    where two of those lie over 26 apart or a byte is 255.  Codes and exponents
+    that begin at any byte."""
+    g = gen(n + k)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8).view(n, k // 32, 16)
+    codes[torch.rand(n, k // 32, generator=g) < 0.5] &= 0x88
+    codes[0] &= 0x88
+    width = torch.randint(1, 40, (n, 1), generator=g)
+    exps = (torch.rand(n, k // 32, generator=g) * width).to(torch.uint8) + torch.randint(0, 210, (n, 1), generator=g, dtype=torch.uint8)
+    exps[torch.rand(n, k // 32, generator=g) < 0.3 / n] = 255
+    want = []
+    for c, e in zip(codes, exps.tolist()):
+        have = [x for x, group in zip(e, c) if bool((group & 0x77).any())]
+        far = 255 in e or (have and max(have) - min(have) > 26)
+        want.append(255 if far else max(have, default=0))
+    codes = codes.view(n, k // 2)
+    assert ops.W4Weight(codes.to(device), exps.to(device)).row_exp.tolist() == want
+    if device == "cuda":
+        for off in (1, 4, 7):
+            c, e = (torch.zeros(t.numel() + off, dtype=torch.uint8, device=device) for t in (codes, exps))
+            c[off:], e[off:] = codes.reshape(-1).to(device), exps.reshape(-1).to(device)
+            assert ops.W4Weight(c[off:].view(n, k // 2), e[off:].view(n, k // 32)).row_exp.tolist() == want
+
+
 def test_w4_weight_leaves_a_loaded_state_alone():
     """A load, an assigning one too, writes nothing into what it was given."""
     for assign in (False, True):
