@@ -726,9 +726,10 @@ class T5ForConditionalGeneration(nn.Module):
                 for i in range(len(caches)):
                     caches[i]["self"]["len"] = 0
                 for t in range(max_new_tokens):
-                    # the 8-bit path reads the fp32 row in place, behind the length too
+                    # fp32 rows, as the attention wants them: one copy for all layers;
+                    # the 8-bit path reads the row in place, behind the length too
                     bias_t = bias_static[:, :, t:t + 1] if kv8 else \
-                        bias_static[:, :, t:t + 1, :t + 1].to(dt).contiguous()
+                        bias_static[:, :, t:t + 1, :t + 1].contiguous()
                     dec = self._decode_step(tok, enc_static, kpad_static, caches, t, bias_t)
                     if cfg.tie_word_embeddings:
                         dec = dec * (self.model_dim**-0.5)
