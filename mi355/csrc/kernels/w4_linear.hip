@@ -18,9 +18,11 @@
 // octaves.  (Smaller ones would be exact as subnormal numbers, but a matrix
 // instruction loses bits of their sum: 6 units of 2^-24 of the sum of sizes at 35
 // octaves, 20 at 36, against 0.7 at up to 30.)  Groups of zeros do not count.
-// Rows that span more, which no quantizer of a trained weight makes, are summed
-// group by group in fp32 by the lanes that store them (far_outputs); their row
-// exponent is given as 255.  Sums are fp32; y is rounded once.
+// Rows that span more, which hardly a trained weight has, are summed group by group
+// in fp32 by the wave that stores them (far_outputs); their row exponent is given
+// as 255.  One of them takes the product of one row by 20480 x 4096 from 12.7 to
+// 13.0 us, of 16 rows by 10240 x 2048 from 8 to 21, of 256 from 25 to 92 (a lane an
+// output: 74, 133, 619).  Sums are fp32; y is rounded once.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -119,14 +121,16 @@ w4_row_exp_kernel(const unsigned char* __restrict__ codes, const unsigned char* 
   if (lane == 0) row_exp[n] = no_scale || most - least > SPAN ? FAR : most;
 }
 
-// One output of such a row: a sum in fp32 for each group, its scale, their sum.
+// One output of such a row, by a wave: a sum in fp32 for each group, a lane a
+// group, at its scale, and their sum.
 template <typename T> DEVINL float far_output(const T* x, const Args& a, int m, int n) {
   const unsigned char* codes = a.codes + (long)n * (a.K >> 1);
   const unsigned char* exps = a.exps + (long)n * (a.K >> 5);
   x += m * a.ldx;
   float sum = 0.f;
 #pragma unroll 1
-  for (int k = 0; k < a.K; k += 32) {
+  for (int k = 32 * (threadIdx.x & 63); k < a.K; k += 32 * 64) {
+    const int e = exps[k >> 5];
     float s = 0.f;
 #pragma unroll 1
     for (int i = k; i < k + 32; i += 8) {
@@ -141,16 +145,23 @@ template <typename T> DEVINL float far_output(const T* x, const Args& a, int m, 
       two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2), 4);
       two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3), 6);
     }
-    const int e = exps[k >> 5];
     sum += e == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(s, e - 127);
   }
-  return sum;
+  return wave_reduce_sum(sum);
 }
 
-// The outputs [m0, m1) of row n, by the lane that stored them.
-template <typename T> DEVINL void far_outputs(const T* x, T* y, const Args& a, int m0, int m1, int n) {
+// The outputs (m, n) of the lanes that are `mine`, one after the other.  Every lane
+// of the wave calls it.
+template <typename T> DEVINL void far_outputs(bool mine, const T* x, T* y, const Args& a, int m, int n) {
+  unsigned long long todo = __ballot(mine);
 #pragma unroll 1
-  for (int m = m0; m < min(m1, a.M); ++m) y[(long)m * a.N + n] = DT<T>::from_f32(far_output(x, a, m, n));
+  while (todo) {
+    const int from = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    const int mm = __builtin_amdgcn_readlane(m, from), nn = __builtin_amdgcn_readlane(n, from);
+    const float sum = far_output(x, a, mm, nn);
+    if ((int)(threadIdx.x & 63) == from) y[(long)mm * a.N + nn] = DT<T>::from_f32(sum);
+  }
 }
 
 // The block's waves hold sums over parts of K, each for the 16 * NT outputs from
@@ -171,14 +182,19 @@ DEVINL void add_waves(f32x4 (*part)[NT][64], const f32x4* acc, int n0, const T* 
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[r] += p[r];
     }
-    if (n >= a.N) continue;
-    const int row_e = a.row_exp[n];
+    const int row_e = a.row_exp[min(n, a.N - 1)];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int m = 4 * (lane >> 4) + r;
-      if (m < a.M) y[(long)m * a.N + n] = DT<T>::from_f32(at_row_scale<T>(s[r], row_e));
+      if (m < a.M && n < a.N) y[(long)m * a.N + n] = DT<T>::from_f32(at_row_scale<T>(s[r], row_e));
     }
-    if (row_e == FAR) far_outputs(x, y, a, 4 * (lane >> 4), 4 * (lane >> 4) + 4, n);
+    if (__any(row_e == FAR)) {
+#pragma unroll 1
+      for (int r = 0; r < 4; ++r) {
+        const int m = 4 * (lane >> 4) + r;
+        far_outputs(row_e == FAR && n < a.N && m < a.M, x, y, a, m, n);
+      }
+    }
   }
 }
 
@@ -265,12 +281,13 @@ __host__ __device__ constexpr int lds_row(int K) { return (K + 255) / 256 * 256 
 // 8 rows 7.3 and 7.5, with 12 rows 10.2 and 7.7.
 // U pieces of 128 lie next to each other.  Eight waves of one piece, but four of
 // two for many outputs and a K under 1024, of which either takes all at once and
-// more, smaller workgroups fill the CUs better: one row by 32128 x 768 5.4 us (6.0
+// more, smaller workgroups fill the CUs better: one row by 32128 x 768 5.0 us (6.0
 // with eight waves), 8 rows 6.9 (7.2), one by 50257 x 768 7.7 (8.0); by 18432 x 768
 // 5.5 and 5.4; by 32128 x 1024 6.9 and 6.8, x 2048 10.7 and 10.4, with 8 rows x 2304
 // 19.6 and 16.3.
+// Registers are held to what leaves room for all 8 waves of a SIMD.
 template <typename T, int NT, int U, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64)
+__global__ void __launch_bounds__(WAVES * 64, 8)
 w4_lds_rows(const T* __restrict__ x, T* __restrict__ y, Args a) {
   using vec = typename Frag<T>::vec;
   __shared__ f32x4 part[WAVES][NT][64];
@@ -486,11 +503,11 @@ w4_many_rows(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ par
   bool far = false;
 #pragma unroll
   for (int u = 0; u < NT; ++u) far |= row_e[u] == FAR;
-  if (far && !part) {                               // w4_add_parts makes them otherwise
+  if (__any(far) && !part) {                        // w4_add_parts makes them otherwise
 #pragma unroll 1
-    for (int i = 0; i < NT * MT; ++i) {
-      const int n = n0 + 16 * (i / MT), m = m_at + wm * 16 * MT + 16 * (i % MT) + 4 * g;
-      if (n < a.N && a.row_exp[n] == FAR) far_outputs(x, y, a, m, m + 4, n);
+    for (int i = 0; i < 4 * NT * MT; ++i) {
+      const int n = n0 + 16 * (i / (4 * MT)), m = m_at + wm * 16 * MT + 16 * (i / 4 % MT) + 4 * g + i % 4;
+      far_outputs(n < a.N && m < a.M && a.row_exp[min(n, a.N - 1)] == FAR, x, y, a, m, n);
     }
   }
 }
@@ -500,12 +517,15 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 w4_add_parts(const T* __restrict__ x, const float* __restrict__ part, T* __restrict__ y, int parts, Args a) {
   const long mn = (long)a.M * a.N, i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= mn) return;
-  float s = 0.f;
+  const bool there = i < mn;
+  const int m = there ? i / a.N : 0, n = there ? i - (long)m * a.N : 0, row_e = a.row_exp[n];
+  if (there) {
+    float s = 0.f;
 #pragma unroll 4
-  for (int p = 0; p < parts; ++p) s += part[p * mn + i];
-  const int m = i / a.N, n = i - (long)m * a.N, row_e = a.row_exp[n];
-  y[i] = DT<T>::from_f32(row_e == FAR ? far_output(x, a, m, n) : at_row_scale<T>(s, row_e));
+    for (int p = 0; p < parts; ++p) s += part[p * mn + i];
+    y[i] = DT<T>::from_f32(at_row_scale<T>(s, row_e));
+  }
+  far_outputs(there && row_e == FAR, x, y, a, m, n);
 }
 
 }  // namespace
