@@ -89,7 +89,9 @@ struct PerSeq {
 // Bound by the bytes it moves: the new tokens are read once into registers,
 // their largest value is found across the group, and codes are written 8 or 16
 // bytes at a time (V through LDS, where it is turned).  512 tokens of 256 x 12
-// heads of 64 in fp16: 126 us, 4.8 TB/s; a large copy reaches 4.9.
+// heads of 64 in fp16: 126 us a call in a stream of them, 4.8 TB/s (a large copy
+// reaches 4.9), 134 and more alone.  8 x 8 chunks of up to 137 tokens, D 128: 7.2 us;
+// K alone 5.1, latency, V alone 6.8.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
@@ -207,7 +209,8 @@ DEVINL unsigned rescale4(unsigned codes, float ratio) {
 // Append of one token, a wave for a (sequence, head) of K or of V: a load, a
 // reduction over the wave and a byte a lane to store.  The codes of the block
 // are touched only if its scale has to grow, which happens to few tokens.
-// Bound by latency: 2.4 us for 12 heads, 4.4 for 256 x 12 (13 as a block).
+// Bound by latency: alone 3.2 us for 12 heads, 5 to 6 for 256 x 12 (as a block 13); a
+// call whose 256 x 12 heads all grow 13.8 us, 9.0 where none does, launch included.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
@@ -307,11 +310,11 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
 // as many outputs land a step beside the nearest one.)  A column's other weights
 // are 0, so mid and lo go there, one column and two columns of the same head
 // further: up to 4 heads take one matrix instruction a tile for all three, up to
-// 8 two, 16 three.  The reference m that is
-// subtracted in the exponent is raised, and what was summed rescaled, only when
-// a score is over it by more than 8: weights then stay under e^8, which costs
-// no precision in fp32 and bf16, and most blocks do without a reduction over
-// the wave.  Scores, statistics and sums are fp32.
+// 8 two, 16 three.  64 x 4 x 8 heads of 128 over 1024 tokens 26.7 us with two, 27.1
+// with three.  The reference m that is subtracted in the exponent is raised, and
+// what was summed rescaled, only when a score is over it by more than 8: weights
+// then stay under e^8, which costs no precision in fp32 and bf16, and most blocks do
+// without a reduction over the wave.  Scores, statistics and sums are fp32.
 //
 // Few rows and a long cache: the blocks of a sequence are dealt to `nsplit`
 // workgroups, whose (o, m, l) a second kernel joins.  Short ones: the four
@@ -320,7 +323,7 @@ kv8_append_one_kernel(const T* __restrict__ knew, const T* __restrict__ vnew, St
 // Bound by the codes' bytes where there are enough of them: 8 x 32 heads of 64
 // over 5000 padded tokens 31 us (5.2 TB/s; a library's sum reads 4.0), 16 x 8
 // x 4 heads of 128 over 8000 to 16384 tokens 80 us (5.0), 256 x 12 heads over
-// 128 tokens 12 us (4.2); 12 heads over 45 tokens 3.9 us, all latency.  With
+// 128 tokens 11.7 us (4.3); 12 heads over 45 tokens 4.1 us, all latency.  With
 // the sixteen weights of a lane made in every column, the first of these took
 // 38 us and the second, whose columns are half used, 77.
 // ---------------------------------------------------------------------------
