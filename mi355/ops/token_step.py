@@ -195,6 +195,7 @@ class KVCache8:
 def kv8_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, start, counts=None) -> None:
     """Write tokens k, v (B, H, S, D) at positions ``start``.. of each sequence.
 
+    On a GPU tokens are bf16 or fp16; a CPU takes any floating type.
     ``start``: a number, or an int32 (B,) tensor.  ``counts``: int32 (B,), how
     many of the S tokens a sequence has (the first ones; default all).  A block
     that was begun keeps the larger of its old scale and what the new tokens
@@ -230,8 +231,8 @@ def decode_attention_kv8(q: torch.Tensor, cache: KVCache8, lengths, bias=None, k
                          scale: float = 1.0, max_len: int | None = None) -> torch.Tensor:
     """Attention of one query token a sequence over a :class:`KVCache8`.
 
-    q: (B, Hq, 1, D), Hq a multiple of the cache's heads (query head i reads
-    cache head i // (Hq/H)).  ``lengths``: a number, or an int32 (B,) tensor
+    q: (B, Hq, 1, D), bf16 or fp16 on a GPU, Hq a multiple of the cache's heads
+    (query head i reads cache head i // (Hq/H)).  ``lengths``: a number, or an int32 (B,) tensor
     that is taken as if clamped to 0..max_len.  ``max_len``: what no length
     exceeds; it sizes the launch (default: the number, or the capacity).
     bias: (1 or B, Hq, 1, >= max_len); kpad: (B, >= max_len) additive: a key
@@ -282,7 +283,8 @@ def check_sampling(temperature, top_k, top_p, min_p) -> None:
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                   min_p=0.0, empty_token: int = -1) -> torch.Tensor:
-    """One token a row of logits (B, V) from given uniform numbers u (B,).
+    """One token a row of logits (B, V), bf16, fp16 or fp32 on a GPU, from given
+    uniform numbers u (B,).
 
     With w = exp((x - max)/temperature) and the order "larger logit first, of
     equal ones the lower index": keep the first ``top_k`` (0: all), of those the
